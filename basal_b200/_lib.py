@@ -13,7 +13,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbasal200.so")
 
-BF16, F16, F32 = 0, 1, 2
+BF16, F16, F32, E4M3 = 0, 1, 2, 3
 DTYPE_CODE = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
 OK, ERR_ARG, ERR_SHAPE, ERR_ALIGN, ERR_DTYPE, ERR_ARCH, ERR_LAUNCH, ERR_TMAP, ERR_LIMIT = range(9)
@@ -51,6 +51,14 @@ SIGNATURES = {
     "basal200_rms_norm_fp8_quant": [_P, _I, _P, _F, _I64, _I64, _P, _P, _P, _P],
     "basal200_gdn_prep": [_P, _I, _I64, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P],
     "basal200_gdn_gate_fp8_quant": [_P, _I, _I, _P, _I, _I64, _I, _P, _F, _I, _I, _I, _P, _P, _P, _P],
+    "basal200_paged_attention": [_P, _I, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _P,
+                                 _I64, _I, _P, _I, _I, _I, _I, _F, _I, _P, _P, _I64, _P],
+    "basal200_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I],
+    "basal200_kv_append": [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _P, _I64,
+                           _I64, _I64, _I, _P, _I64, _I, _P, _P, _I, _I, _I, _I, _P],
+    "basal200_kv_copy_pages": [_P, _P, _P, _I, _I64, _P, _P, _I, _P],
+    "basal200_gdn_step": [_P, _I, _I64, _P, _P, _P, _P, _I, _I, _P, _P, _I64, _I, _I, _I, _P, _P],
+    "basal200_constrain_logits": [_P, _I, _I64, _I, _I, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _P, _I64, _I, _P, _P],
     "basal200_gdn_chunk_rule": [_P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
 
@@ -74,6 +82,7 @@ def lib():
         L.basal200_block_gemm_workspace_bytes.restype = _I64
         L.basal200_block_linear_glu_workspace_bytes.argtypes = [_I64, _I64, _I64]
         L.basal200_block_linear_glu_workspace_bytes.restype = _I64
+        L.basal200_paged_attention_workspace_bytes.restype = _I64
         L.basal200_block_linear_residual_workspace_bytes.argtypes = [_I64, _I64, _I64]
         L.basal200_block_linear_residual_workspace_bytes.restype = _I64
         L.basal200_device_faults.argtypes, L.basal200_device_faults.restype = [_I, _I], ctypes.c_uint

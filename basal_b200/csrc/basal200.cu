@@ -1,6 +1,7 @@
 // libbasal200: host side of the C ABI declared in include/basal200.h, and the one translation unit that holds every
 // kernel of the library (the device fault word is shared by all of them).
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -13,6 +14,9 @@
 #include "readout.cuh"
 #include "hybrid.cuh"
 #include "gdn_chunk.cuh"
+#include "paged.cuh"
+#include "gdn_step.cuh"
+#include "constrain.cuh"
 
 namespace b200 {
 namespace {
@@ -1114,6 +1118,192 @@ int gdn_chunk(const float* q, const float* k, const void* v, int v_dtype, const 
 }
 
 // ------------------------------------------------------------------------------------------------------------
+// One new token a row (paged.cuh, gdn_step.cuh, constrain.cuh)
+// ------------------------------------------------------------------------------------------------------------
+// What the attention and the append ask of a cache's pools and tables.
+int check_cache(int dtype, int kv_dtype, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                const void* ks, const void* vs, int64_t s_page, int64_t s_head, int64_t pages, int page_size,
+                int64_t table_row, int width, int Hk, int D) {
+  if (pages < 0 || page_size <= 0 || width < 0 || Hk <= 0 || table_row < 0) return BASAL200_ERR_ARG;
+  if (page_stride < 0 || head_stride < 0 || token_stride < 0 || s_page < 0 || s_head < 0) return BASAL200_ERR_ARG;
+  if (D != 64 && D != 128 && D != 256) return BASAL200_ERR_SHAPE;
+  if (dtype != BASAL200_BF16 && dtype != BASAL200_F16) return BASAL200_ERR_DTYPE;
+  if (kv_dtype != dtype && kv_dtype != BASAL200_E4M3) return BASAL200_ERR_DTYPE;
+  if (kv_dtype == BASAL200_E4M3 && (!ks || !vs)) return BASAL200_ERR_ARG;
+  const int unit = kv_dtype == BASAL200_E4M3 ? 16 : 8;  // elements of 16 bytes
+  if (page_stride % unit || head_stride % unit || token_stride % unit) return BASAL200_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(ks) & 3) || (reinterpret_cast<uintptr_t>(vs) & 3)) return BASAL200_ERR_ALIGN;
+  if (pages > INT32_MAX || (int64_t)width * page_size > INT32_MAX - 64) return BASAL200_ERR_LIMIT;
+  return BASAL200_OK;
+}
+
+template <typename TQ, typename TK>
+int attend_launch(const paged::AttendParams& p, int D, cudaStream_t st) {
+  const dim3 grid(p.H, p.rows);
+  if (D == 64) return launch_pdl(paged::attend_simple_kernel<TQ, TK, 64>, grid, 128, 0, st, p);
+  if (D == 128) return launch_pdl(paged::attend_simple_kernel<TQ, TK, 128>, grid, 128, 0, st, p);
+  return launch_pdl(paged::attend_simple_kernel<TQ, TK, 256>, grid, 128, 0, st, p);
+}
+
+int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int D, void* workspace,
+                    int64_t workspace_bytes, cudaStream_t st) {
+  if (p.rows < 0 || p.H <= 0 || p.Hk <= 0 || p.window < 0 || p.q_row < 0 || p.q_head < 0) return BASAL200_ERR_ARG;
+  if (p.H % p.Hk) return BASAL200_ERR_SHAPE;
+  int rc = check_cache(q_dtype, kv_dtype, p.page_stride, p.head_stride, p.token_stride, p.ks, p.vs, p.s_page,
+                       p.s_head, p.pages, p.page_size, p.table_row, p.width, p.Hk, D);
+  if (rc) return rc;
+  if (p.rows == 0) return BASAL200_OK;
+  if (!p.q || !p.lengths || !p.out) return BASAL200_ERR_ARG;
+  if ((p.width > 0 && !p.table) || (p.pages > 0 && (!p.k || !p.v))) return BASAL200_ERR_ARG;
+  if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out) || p.q_row % 8 || p.q_head % 8)
+    return BASAL200_ERR_ALIGN;
+  if (p.rows > 65535) return BASAL200_ERR_LIMIT;
+  int dev;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  using bf16 = __nv_bfloat16;
+  if (q_dtype == BASAL200_BF16)
+    return kv_dtype == BASAL200_E4M3 ? attend_launch<bf16, uint8_t>(p, D, st) : attend_launch<bf16, bf16>(p, D, st);
+  return kv_dtype == BASAL200_E4M3 ? attend_launch<__half, uint8_t>(p, D, st) : attend_launch<__half, __half>(p, D, st);
+}
+
+template <typename T, bool FP8>
+int append_launch(const paged::AppendParams& p, int D, cudaStream_t st) {
+  const int64_t grid = ((int64_t)p.rows * p.T * p.Hk * 2 + 7) / 8;  // a warp each, 8 a CTA
+  if (grid > INT32_MAX) return BASAL200_ERR_LIMIT;
+  if (D == 64) return launch_pdl(paged::append_kernel<T, FP8, 64>, (unsigned)grid, 256, 0, st, p);
+  if (D == 128) return launch_pdl(paged::append_kernel<T, FP8, 128>, (unsigned)grid, 256, 0, st, p);
+  return launch_pdl(paged::append_kernel<T, FP8, 256>, (unsigned)grid, 256, 0, st, p);
+}
+
+int kv_append(const paged::AppendParams& p, int dtype, int kv_dtype, int D, cudaStream_t st) {
+  if (p.rows < 0 || p.T < 0) return BASAL200_ERR_ARG;
+  int rc = check_cache(dtype, kv_dtype, p.page_stride, p.head_stride, p.token_stride, p.scale[0], p.scale[1],
+                       p.s_page, p.s_head, p.pages, p.page_size, p.table_row, p.width, p.Hk, D);
+  if (rc) return rc;
+  if (p.rows == 0 || p.T == 0) return BASAL200_OK;
+  if (!p.start || (p.width > 0 && !p.table)) return BASAL200_ERR_ARG;
+  for (int i = 0; i < 2; ++i) {
+    if (!p.src[i] || (p.pages > 0 && !p.pool[i]) || p.row[i] < 0 || p.tok[i] < 0 || p.head[i] < 0)
+      return BASAL200_ERR_ARG;
+    if (!aligned16(p.src[i]) || !aligned16(p.pool[i]) || p.row[i] % 8 || p.tok[i] % 8 || p.head[i] % 8)
+      return BASAL200_ERR_ALIGN;
+  }
+  int dev;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  const bool fp8 = kv_dtype == BASAL200_E4M3;
+  if (dtype == BASAL200_BF16)
+    return fp8 ? append_launch<__nv_bfloat16, true>(p, D, st) : append_launch<__nv_bfloat16, false>(p, D, st);
+  return fp8 ? append_launch<__half, true>(p, D, st) : append_launch<__half, false>(p, D, st);
+}
+
+// Whether every index is in [0, pages), no page is written twice and none is both read and written. A bitmap of the
+// pages' roles where the list is long (calloc: nothing here throws); false too when it cannot be had.
+bool moves_are_apart(const int32_t* src, const int32_t* dst, int n, int64_t pages) {
+  for (int i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages) return false;
+  if (n <= 32) {
+    for (int i = 0; i < n; ++i)
+      for (int j = 0; j < n; ++j)
+        if (src[j] == dst[i] || (j != i && dst[j] == dst[i])) return false;
+    return true;
+  }
+  uint8_t* written = static_cast<uint8_t*>(calloc((size_t)pages / 8 + 1, 1));
+  if (!written) return false;
+  bool ok = true;
+  for (int i = 0; i < n && ok; ++i) {
+    const uint8_t bit = (uint8_t)(1u << (dst[i] & 7));
+    ok = !(written[dst[i] >> 3] & bit);
+    written[dst[i] >> 3] |= bit;
+  }
+  for (int i = 0; i < n && ok; ++i) ok = !(written[src[i] >> 3] >> (src[i] & 7) & 1);
+  free(written);
+  return ok;
+}
+
+template <int N>
+int copy_pages_launch(void* const* pools, const int* layers, const int64_t* page_bytes, int npools, int64_t pages,
+                      const int32_t* src, const int32_t* dst, int n, cudaStream_t st) {
+  paged::CopyParams<N> p;
+  int most = 0;
+  for (int i = 0; i < npools; ++i) {
+    p.pool[i] = static_cast<char*>(pools[i]);
+    p.page_bytes[i] = page_bytes[i];
+    p.layer_bytes[i] = page_bytes[i] * pages;
+    p.layers[i] = layers[i];
+    if (layers[i] > most) most = layers[i];
+  }
+  if (!most) return BASAL200_OK;
+  for (int at = 0; at < n; at += N) {
+    p.n = n - at < N ? n - at : N;
+    memcpy(p.src, src + at, (size_t)p.n * 4);
+    memcpy(p.dst, dst + at, (size_t)p.n * 4);
+    const int rc = launch_pdl(paged::copy_pages_kernel<N>, dim3(p.n, most, npools), 256, 0, st, p);
+    if (rc) return rc;
+  }
+  return BASAL200_OK;
+}
+
+int kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_bytes, int npools, int64_t pages,
+                  const int32_t* src, const int32_t* dst, int n, cudaStream_t st) {
+  if (npools < 0 || n < 0 || pages < 0) return BASAL200_ERR_ARG;
+  if (npools > paged::kCopyPools || pages > INT32_MAX) return BASAL200_ERR_LIMIT;
+  if (npools == 0 || n == 0) return BASAL200_OK;
+  if (!pools || !layers || !page_bytes || !src || !dst) return BASAL200_ERR_ARG;
+  for (int i = 0; i < npools; ++i) {
+    if (!pools[i] || layers[i] < 0 || page_bytes[i] <= 0) return BASAL200_ERR_ARG;
+    if (layers[i] > 65535) return BASAL200_ERR_LIMIT;
+    if ((reinterpret_cast<uintptr_t>(pools[i]) & 3) || page_bytes[i] % 4) return BASAL200_ERR_ALIGN;
+  }
+  if (!moves_are_apart(src, dst, n, pages)) return BASAL200_ERR_ARG;
+  int dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  if (n <= 32) return copy_pages_launch<32>(pools, layers, page_bytes, npools, pages, src, dst, n, st);
+  return copy_pages_launch<1024>(pools, layers, page_bytes, npools, pages, src, dst, n, st);
+}
+
+int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
+  if (p.rows < 0 || p.Hk <= 0 || p.Hv <= 0 || p.slots < 0) return BASAL200_ERR_ARG;
+  if (p.Hv % p.Hk) return BASAL200_ERR_SHAPE;
+  if (dt != BASAL200_BF16 && dt != BASAL200_F16) return BASAL200_ERR_DTYPE;
+  if (p.rows == 0) return BASAL200_OK;
+  if (!p.proj || !p.conv || !p.A_log || !p.dt_bias || !p.o || (p.slots > 0 && (!p.tail || !p.state)))
+    return BASAL200_ERR_ARG;
+  const int64_t C = (int64_t)(2 * p.Hk + p.Hv) * 128;
+  if (p.ld < C || p.b_off < 0 || p.a_off < 0 || (int64_t)p.b_off + p.Hv > p.ld || (int64_t)p.a_off + p.Hv > p.ld)
+    return BASAL200_ERR_SHAPE;
+  if (!aligned16(p.state) || !aligned16(p.conv) || !aligned16(p.o) || (p.ld % 4) ||
+      (reinterpret_cast<uintptr_t>(p.proj) & 7) || (reinterpret_cast<uintptr_t>(p.tail) & 7))
+    return BASAL200_ERR_ALIGN;
+  if (p.rows > 65535 || p.Hv > 65535 / 128) return BASAL200_ERR_LIMIT;
+  int dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  if (dt == BASAL200_BF16)
+    return launch_pdl(gdnstep::gdn_step_kernel<__nv_bfloat16>, dim3(p.Hk, p.rows), 128, 0, st, p);
+  return launch_pdl(gdnstep::gdn_step_kernel<__half>, dim3(p.Hk, p.rows), 128, 0, st, p);
+}
+
+int constrain_logits(const constrain::Params& p, int dt, cudaStream_t st) {
+  if (p.rows < 0 || p.V < 0 || p.T < 0 || p.N < 0 || p.ld < 0 || p.mask_row < 0 || p.past_row < 0 || p.bias_row < 0)
+    return BASAL200_ERR_ARG;
+  if (dt != BASAL200_BF16 && dt != BASAL200_F16 && dt != BASAL200_F32) return BASAL200_ERR_DTYPE;
+  if (p.rows == 0 || p.V == 0) return BASAL200_OK;
+  if (!p.logits || !p.out || (p.T > 0 && !p.past) || (p.N > 0 && (!p.ids || !p.values))) return BASAL200_ERR_ARG;
+  if (!aligned16(p.out)) return BASAL200_ERR_ALIGN;
+  if (p.rows > 65535 || p.V > (1 << 30) || p.N > 4096) return BASAL200_ERR_LIMIT;
+  int dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  const dim3 grid((p.V + constrain::SLICE - 1) / constrain::SLICE, p.rows);
+  if (dt == BASAL200_BF16) return launch_pdl(constrain::constrain_kernel<__nv_bfloat16>, grid, 256, 0, st, p);
+  if (dt == BASAL200_F16) return launch_pdl(constrain::constrain_kernel<__half>, grid, 256, 0, st, p);
+  return launch_pdl(constrain::constrain_kernel<float>, grid, 256, 0, st, p);
+}
+
+// ------------------------------------------------------------------------------------------------------------
 // Allocation-free FP8-block linear: the activation codes and scales live in one file-scope device array instead of
 // caller scratch. The array is part of the loaded module, so every GPU that loads the library holds its
 // 16.5 MiB until the process exits; all calls on a device share it.
@@ -1320,6 +1510,136 @@ int basal200_gdn_chunk_rule(const float* q, const float* k, const void* v, int v
 // The two kernels of basal200_fp8_block_linear, the quantiser writing into the library's own device array. Nothing
 // there needs clearing between calls: the quantiser writes every code and scale the GEMM then reads, and rows past M
 // are zero-filled by the GEMM's TMA loads, never read from the array.
+int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t q_head, const void* k, const void* v,
+                             int kv_dtype, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                             const float* ks, const float* vs, int64_t s_page, int64_t s_head, int64_t pages,
+                             int page_size, const int32_t* table, int64_t table_row, int width,
+                             const int32_t* lengths, int rows, int H, int Hk, int D, float scale, int window,
+                             void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  b200::paged::AttendParams p = {};
+  p.q = q;
+  p.q_row = q_row;
+  p.q_head = q_head;
+  p.k = k;
+  p.v = v;
+  p.page_stride = page_stride;
+  p.head_stride = head_stride;
+  p.token_stride = token_stride;
+  p.ks = ks;
+  p.vs = vs;
+  p.s_page = s_page;
+  p.s_head = s_head;
+  p.pages = pages;
+  p.page_size = page_size;
+  p.table = table;
+  p.table_row = table_row;
+  p.width = width;
+  p.lengths = lengths;
+  p.rows = rows;
+  p.H = H;
+  p.Hk = Hk;
+  p.scale = scale;
+  p.window = window;
+  p.out = out;
+  return b200::paged_attention(p, q_dtype, kv_dtype, D, workspace, workspace_bytes, as_stream(stream));
+}
+
+int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int width, int page_size,
+                                                 int window) {
+  return 0;
+}
+
+int basal200_kv_append(const void* k, const void* v, int dtype, int64_t k_row, int64_t k_tok, int64_t k_head,
+                       int64_t v_row, int64_t v_tok, int64_t v_head, void* k_pool, void* v_pool, int kv_dtype,
+                       int64_t page_stride, int64_t head_stride, int64_t token_stride, float* ks, float* vs,
+                       int64_t s_page, int64_t s_head, int64_t pages, int page_size, const int32_t* table,
+                       int64_t table_row, int width, const int32_t* start, const int32_t* count, int rows, int T,
+                       int Hk, int D, void* stream) {
+  b200::paged::AppendParams p = {};
+  p.src[0] = k;
+  p.src[1] = v;
+  p.row[0] = k_row;
+  p.row[1] = v_row;
+  p.tok[0] = k_tok;
+  p.tok[1] = v_tok;
+  p.head[0] = k_head;
+  p.head[1] = v_head;
+  p.pool[0] = k_pool;
+  p.pool[1] = v_pool;
+  p.page_stride = page_stride;
+  p.head_stride = head_stride;
+  p.token_stride = token_stride;
+  p.scale[0] = ks;
+  p.scale[1] = vs;
+  p.s_page = s_page;
+  p.s_head = s_head;
+  p.pages = pages;
+  p.page_size = page_size;
+  p.table = table;
+  p.table_row = table_row;
+  p.width = width;
+  p.start = start;
+  p.count = count;
+  p.rows = rows;
+  p.T = T;
+  p.Hk = Hk;
+  return b200::kv_append(p, dtype, kv_dtype, D, as_stream(stream));
+}
+
+int basal200_kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_bytes, int npools,
+                           int64_t pages, const int32_t* src, const int32_t* dst, int n, void* stream) {
+  return b200::kv_copy_pages(pools, layers, page_bytes, npools, pages, src, dst, n, as_stream(stream));
+}
+
+int basal200_gdn_step(const void* proj, int dtype, int64_t ld, void* tail, const void* conv, const float* A_log,
+                      const void* dt_bias, int b_off, int a_off, float* state, const int32_t* at, int64_t slots,
+                      int rows, int Hk, int Hv, void* o, void* stream) {
+  b200::gdnstep::Params p = {};
+  p.proj = proj;
+  p.ld = ld;
+  p.tail = tail;
+  p.conv = conv;
+  p.A_log = A_log;
+  p.dt_bias = dt_bias;
+  p.b_off = b_off;
+  p.a_off = a_off;
+  p.state = state;
+  p.at = at;
+  p.slots = slots;
+  p.rows = rows;
+  p.Hk = Hk;
+  p.Hv = Hv;
+  p.q_scale = 0.08838834764831845f;  // 128^-1/2, as basal200_gdn_prep's
+  p.o = o;
+  return b200::gdn_step(p, dtype, as_stream(stream));
+}
+
+int basal200_constrain_logits(const void* logits, int dtype, int64_t ld, int rows, int V, const uint32_t* mask,
+                              int64_t mask_row, const int32_t* past, int64_t past_row, int T,
+                              const float* repetition, const float* presence, const float* frequency,
+                              const int32_t* ids, const float* values, int64_t bias_row, int N, float* out,
+                              void* stream) {
+  b200::constrain::Params p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = rows;
+  p.V = V;
+  p.mask = mask;
+  p.mask_row = mask_row;
+  p.past = past;
+  p.past_row = past_row;
+  p.T = T;
+  p.repetition = repetition;
+  p.presence = presence;
+  p.frequency = frequency;
+  p.ids = ids;
+  p.values = values;
+  p.bias_row = bias_row;
+  p.N = N;
+  p.out = out;
+  return b200::constrain_logits(p, dtype, as_stream(stream));
+}
+
 int basal200_fp8_block_linear_noalloc(const void* x, int x_dtype, const uint8_t* w, const float* ws,
                                       const void* bias, void* y, int64_t M, int64_t N, int64_t K, void* stream) {
   if (M < 0 || K <= 0) return BASAL200_ERR_ARG;

@@ -18,6 +18,8 @@ enum FaultBits : unsigned {
   kFaultTimeoutDrain = BASAL200_FAULT_TIMEOUT_DRAIN,
   kFaultBadId = BASAL200_FAULT_BAD_ID,
   kFaultTimeoutPeer = BASAL200_FAULT_TIMEOUT_PEER,
+  kFaultBadPage = BASAL200_FAULT_BAD_PAGE,
+  kFaultBadSlot = BASAL200_FAULT_BAD_SLOT,
 };
 
 // The library is one translation unit (csrc/basal200.cu includes every kernel header), so the word is defined here.

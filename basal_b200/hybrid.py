@@ -11,6 +11,9 @@ FP8-block BlockFP8Linear of this package, answering decision requests with the o
       .suffix_hidden(ids, st)   rows [B, S] that continue the prefix -> the final-normed hidden state of each row's
                         last token [B, D]
       .decide(ids, st, readout, rows, idx, pad)   -> option probabilities [B, k]
+      .open(ids, st, tokens)    the same suffix pass, kept so that the rows can go on token by token -> StepState
+      .step(ids, s)             one new token a row [B] -> its final-normed hidden state [B, D]
+      .answer(ids, st, steps, ...)   greedy answers of several tokens under penalties, biases and grammar masks
 
 The linears are basal::fp8_block_linear (the projections that read one input merged into one weight, as
 blockquant.fuse does for the reference: the Gated DeltaNet's q/k/v/z/b/a, the attention's q+gate/k/v), the gated MLP
@@ -18,7 +21,10 @@ input basal::fp8_block_linear_glu (SwiGLU in the GEMM's epilogue) and the output
 basal::fp8_block_linear_residual (the residual add in the GEMM's epilogue). The norms, the convolution, the gates and
 the rotary embedding follow the reference's roundings (bf16 between operations, fp32 inside the norms); the
 recurrence runs in fp32 over chunks of 64 tokens (basal::gdn_chunk_rule); the attention over the prefix and the rows'
-own tokens is torch's scaled_dot_product_attention. Everything runs on the GPU.
+own tokens is torch's scaled_dot_product_attention. Token by token, the attention's keys and values live in a paged
+cache whose prefix pages the rows share (kvcache.PagedKVCache: basal::kv_append, basal::paged_attention), the Gated
+DeltaNet takes one token at a time (basal::gdn_step), and the next token is chosen from logits under penalties and
+masks (basal::constrain_logits). Everything runs on the GPU.
 """
 import dataclasses
 import math
@@ -28,6 +34,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .fp8block import BlockFP8Linear
+from .kvcache import PagedKVCache
 
 LINEAR, FULL = "linear_attention", "full_attention"
 
@@ -124,6 +131,18 @@ class PrefixState:
             vb[:, :, :P].copy_(pv.expand(b, -1, -1, -1))
             self.buffers[(i, T)] = kb, vb
         return kb[:b], vb[:b]
+
+
+@dataclasses.dataclass
+class StepState:
+    """Rows that go on token by token: their sequences in the paged cache, per Gated DeltaNet layer the states [B, value
+    heads, 128, 128] fp32 and convolution inputs [B, 3, channels] (both updated in place), the next token's position
+    and the final-normed hidden state [B, D] of each row's last token."""
+    cache: PagedKVCache
+    seqs: list
+    states: list
+    position: int
+    hidden: torch.Tensor
 
 
 class HybridClassifier:
@@ -290,6 +309,103 @@ class HybridClassifier:
     def decide(self, ids, st, readout, rows, idx, pad):
         """Option probabilities [B, k] of the rows' last tokens: the readout of readout.rows(...) = rows, idx, pad."""
         return readout.device_probs(self.suffix_hidden(ids, st), rows, idx, pad)
+
+    @torch.no_grad()
+    def open(self, ids, st, tokens, page_size=64, fp8=False):
+        """The suffix pass of rows ids [B, S] after the prefix st, kept -> StepState with room for `tokens` more tokens
+        a row. The rows' keys and values go to a paged cache (8-bit pages when fp8) whose prefix pages they share."""
+        cfg = self.cfg
+        B, S = ids.shape
+        if B < 1 or S < 1 or tokens < 0:
+            raise ValueError(f"open: rows of at least one token and tokens >= 0, not {list(ids.shape)}, {tokens}")
+        P = st.length
+        pos = torch.arange(P, P + S, device=self.device)[None].expand(B, S)
+        h, kv, states = self._layers(ids.to(self.device), pos, st)
+        own = -(-(P % page_size + S + tokens) // page_size)  # a row's pages past the prefix's full ones
+        cache = PagedKVCache(max(1, len(kv)), -(-P // page_size) + B * own, cfg.kv_heads, cfg.head_dim, page_size,
+                             self.dtype, fp8, self.device)
+        base = cache.add()
+        cache.grow([base], P)
+        for i, (k, v) in enumerate(st.kv):
+            cache.append(i, cache.batch([base]), k.transpose(1, 2), v.transpose(1, 2))
+        seqs = [cache.fork(base) for _ in range(B)]
+        cache.free(base)
+        cache.grow(seqs, S)
+        batch = cache.batch(seqs)
+        for i, (k, v) in enumerate(kv):
+            cache.append(i, batch, k.transpose(1, 2), v.transpose(1, 2))
+        return StepState(cache, seqs, states, P + S, rms(h[:, -1], self.final_norm, cfg.eps))
+
+    def _gdn_step(self, L, h, state, tail):
+        """_gdn for one token a row h [B, D]: the input steps and the recurrence are one kernel, which updates state
+        and tail in place."""
+        cfg = self.cfg
+        B = h.shape[0]
+        q8, s8 = ops.rms_norm_fp8_quant(h, L["nw"], cfg.eps)
+        w_in = L["w_in"]
+        proj = ops.fp8_block_gemm(q8, s8, w_in.weight, w_in.weight_scale, h.dtype)
+        b_off = cfg.conv_dim + cfg.value_dim
+        o = ops.gdn_step(proj, tail, L["conv"], L["A_log"], L["dt_bias"], state, cfg.lin_k_heads, cfg.lin_v_heads,
+                         b_off, b_off + cfg.lin_v_heads)
+        qo, so = ops.gdn_gate_fp8_quant(o, proj, cfg.conv_dim, L["gnorm"], cfg.eps, B, 1)
+        out = L["out"]
+        return ops.fp8_block_gemm_residual(qo, so, out.weight, out.weight_scale, None, h)
+
+    def _attention_step(self, L, h, cos, sin, cache, layer, batch):
+        """_attention for one token a row h [B, D] over the paged cache, its key and value appended first."""
+        cfg = self.cfg
+        B, H, Hk, d = h.shape[0], cfg.heads, cfg.kv_heads, cfg.head_dim
+        q8, s8 = ops.rms_norm_fp8_quant(h, L["nw"], cfg.eps)
+        w = L["w_qkv"]
+        qkv = ops.fp8_block_gemm(q8, s8, w.weight, w.weight_scale, h.dtype)
+        k, v = h.new_empty(B, Hk, 1, d), h.new_empty(B, Hk, 1, d)
+        q = ops.attn_prep(qkv, L["q_norm"], L["k_norm"], cfg.eps, cos, sin, cfg.rotary_dims, H, Hk, B, 1, k, v, 0)
+        cache.append(layer, batch, k.transpose(1, 2), v.transpose(1, 2))
+        o = cache.attend(layer, batch, q.view(B, H, d), 1.0 / math.sqrt(d))
+        qa, sa = ops.attn_gate_fp8_quant(o.view(B, H, 1, d), qkv, B, 1, H)
+        out = L["o"]
+        return ops.fp8_block_gemm_residual(qa, sa, out.weight, out.weight_scale, out.bias, h)
+
+    @torch.no_grad()
+    def step(self, ids, s):
+        """One new token a row, ids [B], after what s holds -> final-normed hidden states [B, D] (s.hidden too)."""
+        if ids.shape != (len(s.seqs),):
+            raise ValueError(f"step: one token for each of {len(s.seqs)} rows, not {list(ids.shape)}")
+        s.cache.grow(s.seqs)
+        batch = s.cache.batch(s.seqs)
+        h = self.embed[ids.to(self.device)]
+        cos, sin = rope_tables(self.cfg, torch.full((1, 1), s.position, device=self.device), h.dtype)
+        ia = ig = 0
+        for L in self.layers:
+            if L["kind"] == LINEAR:
+                h = self._gdn_step(L, h, *s.states[ig])
+                ig += 1
+            else:
+                h = self._attention_step(L, h, cos, sin, s.cache, ia, batch)
+                ia += 1
+            h = self._mlp(L, h[:, None])[:, 0]
+        s.position += 1
+        s.hidden = rms(h, self.final_norm, self.cfg.eps)
+        return s.hidden
+
+    @torch.no_grad()
+    def answer(self, ids, st, steps, mask=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+               bias_values=None, page_size=64, fp8=False):
+        """Greedy answers of `steps` tokens after rows ids [B, S] -> int64 [B, steps]. Each step's logits (the LM head
+        over the whole vocabulary) go through basal::constrain_logits with the row's answer so far as its history.
+        mask: None, a bit mask [1 or B, ceil(vocab / 32)] for every step, or a function of the answer so far (int32
+        [B, t]) that returns the step's mask. repetition, presence, frequency: fp32 [B] or None."""
+        s = self.open(ids, st, max(0, steps - 1), page_size, fp8)
+        B = len(s.seqs)
+        past = torch.full((B, max(1, steps)), -1, dtype=torch.int32, device=self.device)
+        for t in range(steps):
+            if t:
+                self.step(past[:, t - 1].long(), s)
+            now = mask(past[:, :t]) if callable(mask) else mask
+            z = ops.constrain_logits(F.linear(s.hidden, self.head.weight), now, past, repetition, presence, frequency,
+                                     bias_ids, bias_values)
+            past[:, t] = z.argmax(-1)
+        return past[:, :steps].long()
 
     def linears(self):
         """Every FP8-block linear of the model, with its name."""

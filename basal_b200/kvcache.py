@@ -1,0 +1,179 @@
+"""A paged key / value cache: the pages of every attention layer, which sequence holds which of them, and forks that
+share them. The reference answers from one prefill pass and keeps whole key / value buffers; a model that goes on from
+there token by token (hybrid.HybridClassifier.open / step / answer) keeps its keys and values here.
+
+  PagedKVCache(layers, pages, kv_heads, head_dim, page_size, dtype, fp8, device)
+      .add()                  a new, empty sequence -> its number
+      .fork(seq)              a new sequence with seq's tokens, its pages shared and counted (nothing is copied)
+      .grow(seqs, n)          room for n more tokens in each of seqs: new pages, and a copy of a shared page before it
+                              is written (one basal::kv_copy_pages over every layer); raises MemoryError, with nothing
+                              changed, when the free pages do not suffice
+      .batch(seqs)            -> Batch: the sequences' table and lengths on the device, for append and attend
+      .append(layer, batch, k, v), .attend(layer, batch, q, scale, window)
+                              basal::kv_append of the tokens that grow() made room for, basal::paged_attention
+      .free(seq)              gives its pages back
+      .compact()              moves the live pages to the lowest numbers (one kv_copy_pages) -> how many pages are live
+
+The bookkeeping is on the host; the device sees the pages, and tables and lengths as int32 tensors.
+"""
+import dataclasses
+
+import torch
+
+from . import ops
+
+E4M3 = torch.float8_e4m3fn
+
+
+@dataclasses.dataclass
+class Batch:
+    """Some sequences, in order, as the kernels see them: table [rows, width], the lengths [rows] with the tokens that
+    the last grow() made room for, and where those begin."""
+    seqs: list
+    table: torch.Tensor
+    lengths: torch.Tensor
+    start: torch.Tensor
+    count: torch.Tensor
+
+
+class PagedKVCache:
+    def __init__(self, layers, pages, kv_heads, head_dim, page_size=64, dtype=torch.bfloat16, fp8=False,
+                 device="cuda"):
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"PagedKVCache: heads of 64, 128 or 256, not {head_dim}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"PagedKVCache: keys and values of bfloat16 or float16, not {dtype}")
+        if min(layers, pages, kv_heads, page_size) <= 0:
+            raise ValueError("PagedKVCache: layers, pages, kv_heads and page_size must be positive")
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        self.device = torch.device(device)
+        self.page_size, self.pages, self.dtype = page_size, pages, dtype
+        self.k = torch.empty(shape, dtype=E4M3 if fp8 else dtype, device=self.device)
+        self.v = torch.empty_like(self.k)
+        self.k_scale = torch.empty(shape[:4], dtype=torch.float32, device=self.device) if fp8 else None
+        self.v_scale = torch.empty_like(self.k_scale) if fp8 else None
+        self._free = list(range(pages - 1, -1, -1))
+        self._shares = [0] * pages   # sequences that hold a page
+        self._of = {}                # sequence -> its pages, in order
+        self._length = {}
+        self._new = {}               # tokens that the last grow() made room for
+        self._next = 0
+
+    @property
+    def pools(self):
+        return [p for p in (self.k, self.v, self.k_scale, self.v_scale) if p is not None]
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _known(self, seq):
+        if seq not in self._of:
+            raise KeyError(f"PagedKVCache: no sequence {seq}")
+        return self._of[seq]
+
+    def length(self, seq):
+        self._known(seq)
+        return self._length[seq]
+
+    def pages_of(self, seq):
+        return list(self._known(seq))
+
+    def add(self):
+        seq, self._next = self._next, self._next + 1
+        self._of[seq], self._length[seq], self._new[seq] = [], 0, 0
+        return seq
+
+    def fork(self, seq):
+        pages = self._known(seq)
+        new = self.add()
+        self._of[new], self._length[new] = list(pages), self._length[seq]
+        for p in pages:
+            self._shares[p] += 1
+        return new
+
+    def free(self, seq):
+        for p in self._known(seq):
+            self._shares[p] -= 1
+            if not self._shares[p]:
+                self._free.append(p)
+        del self._of[seq], self._length[seq], self._new[seq]
+
+    def grow(self, seqs, n=1):
+        """n: tokens for each sequence, a number or a list."""
+        seqs = list(seqs)
+        n = [n] * len(seqs) if isinstance(n, int) else list(n)
+        if len(n) != len(seqs) or len(set(seqs)) != len(seqs) or min(n, default=0) < 0:
+            raise ValueError("PagedKVCache: grow takes each sequence once, with its number of tokens")
+        # the shared page that a sequence writes into next is replaced by a copy; of the sequences that share a page
+        # and all write it, the last keeps it
+        left, copies, need = {}, [], 0
+        for s, m in zip(seqs, n):
+            pages, length = self._known(s), self._length[s]
+            if m and length % self.page_size:
+                p = pages[length // self.page_size]
+                if left.get(p, self._shares[p]) > 1:
+                    left[p] = left.get(p, self._shares[p]) - 1
+                    copies.append(s)
+                    need += 1
+            need += max(0, -(-(length + m) // self.page_size) - len(pages))
+        if need > len(self._free):
+            raise MemoryError(f"PagedKVCache: {need} pages are needed, {len(self._free)} are free")
+        src, dst = [], []
+        for s in copies:
+            at = self._length[s] // self.page_size
+            old, new = self._of[s][at], self._free.pop()
+            self._shares[old] -= 1
+            self._shares[new] = 1
+            self._of[s][at] = new
+            src.append(old)
+            dst.append(new)
+        if src:
+            ops.kv_copy_pages(self.pools, src, dst)
+        for s, m in zip(seqs, n):
+            pages = self._of[s]
+            while len(pages) * self.page_size < self._length[s] + m:
+                pages.append(self._free.pop())
+                self._shares[pages[-1]] = 1
+            self._length[s] += m
+            self._new[s] = m
+
+    def batch(self, seqs):
+        seqs = list(seqs)
+        width = max([len(self._known(s)) for s in seqs], default=0) or 1
+        rows = []
+        for s in seqs:
+            rows.append(self._of[s] + [-1] * (width - len(self._of[s])) +
+                        [self._length[s], self._length[s] - self._new[s], self._new[s]])
+        host = torch.tensor(rows, dtype=torch.int32).view(len(seqs), width + 3)
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        t = host.to(self.device, non_blocking=True)
+        lengths, start, count = t[:, width:].t().contiguous()
+        return Batch(seqs, t[:, :width], lengths, start, count)
+
+    def _layer(self, i):
+        return (self.k[i], self.v[i]), (None, None) if self.k_scale is None else (self.k_scale[i], self.v_scale[i])
+
+    def append(self, layer, batch, k, v):
+        (pk, pv), (ks, vs) = self._layer(layer)
+        ops.kv_append(k, v, pk, pv, batch.table, batch.start, batch.count, ks, vs)
+
+    def attend(self, layer, batch, q, scale, window=0):
+        (pk, pv), (ks, vs) = self._layer(layer)
+        return ops.paged_attention(q, pk, pv, batch.table, batch.lengths, scale, window, ks, vs)
+
+    def compact(self):
+        live = [p for p in range(self.pages) if self._shares[p]]
+        n = len(live)
+        holes = [p for p in range(n) if not self._shares[p]]
+        movers = [p for p in live if p >= n]  # as many as there are holes below n
+        if movers:
+            ops.kv_copy_pages(self.pools, movers, holes)
+            to = dict(zip(movers, holes))
+            for pages in self._of.values():
+                pages[:] = [to.get(p, p) for p in pages]
+            for a, b in to.items():
+                self._shares[b], self._shares[a] = self._shares[a], 0
+        self._free = list(range(self.pages - 1, n - 1, -1))
+        return n

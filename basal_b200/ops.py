@@ -33,12 +33,25 @@
   basal::attn_prep(qkv, q_norm, k_norm, eps, cos, sin, rot, H, Hk, rows, T, k_buf, v_buf, kv_off)
                                                  the attention's q / k norms and rotary embedding (gdn_graph.py:452-460)
   basal::attn_gate_fp8_quant(o, qkv, rows, T, H) its output gate fused with the FP8 quantiser (gdn_graph.py:464-466)
+  basal::paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)
+                                                 attention of one new token a row over a paged key / value cache
+  basal::kv_append(k, v, k_pages, v_pages, table, start, count, k_scale, v_scale)
+                                                 new tokens' keys and values into the cache's pages
+  basal::kv_copy_pages(pools, src, dst)          pages copied within a cache, every layer at once
+  basal::gdn_step(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots)
+                                                 the Gated DeltaNet for one new token a row, its state in place
+  basal::constrain_logits(logits, mask, past, repetition, presence, frequency, bias_ids, bias_values)
+                                                 penalties, biases and a grammar mask on a step's logits
+                                                 (these five have no counterpart in the reference, which answers
+                                                 from one prefill pass)
 
-Every op but attn_prep is functional (mutates_args=(); attn_prep writes the keys and values into the buffers it is
-given), allocates its outputs (and scratch) from the caching allocator, enqueues on
+Every op but attn_prep, kv_append, kv_copy_pages and gdn_step is functional (mutates_args=(); attn_prep writes the keys
+and values into the buffers it is given, kv_append and kv_copy_pages into the cache's pages, gdn_step into its state
+and tail), allocates its outputs (and scratch) from the caching allocator, enqueues on
 the current stream and never synchronises: Dynamo traces them through their fake kernels and a CUDA graph captures
 their launches. They need CUDA tensors; there is no CPU implementation.
 """
+import ctypes
 from typing import Optional
 
 import torch
@@ -613,3 +626,272 @@ def _(q, k, v, g, beta, s0, o_16bit=False):
     rows, H = v.shape[0], v.shape[1]
     o_dtype = v.dtype if o_16bit and v.dtype != torch.float32 else torch.float32
     return q.new_empty(v.shape, dtype=o_dtype), q.new_empty((rows, H, 128, 128), dtype=torch.float32)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# one new token a row: the paged key / value cache, the recurrent state, the next token's logits
+# ---------------------------------------------------------------------------------------------------------------
+_STEP = torch.library.Library("basal", "FRAGMENT")
+
+
+def _step_op(schema, fake=None):
+    """Defines basal::<schema> with the decorated function as its implementation and returns the op. A step's calls
+    are short (a few microseconds of device time), so these ops are registered without torch.library.custom_op's
+    wrappers: 4 instead of 13 us of host time a call."""
+    name = schema.split("(")[0]
+
+    def wrap(f):
+        _STEP.define(schema)
+        for key in ("CUDA", "CPU"):  # CPU tensors reach the function's own checks
+            _STEP.impl(name, f, key)
+        torch.library.register_fake(f"basal::{name}", fake or (lambda *a: None), lib=_STEP)
+        return getattr(torch.ops.basal, name).default
+
+    return wrap
+
+
+def _on(dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            require_cuda(t)
+            raise ValueError(f"basal_b200: a tensor is on {t.device}, another on {dev}")
+
+
+def _int32(what, t, *shape):
+    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{what} must be int32 {['any' if n is None else n for n in shape]}, not {t.dtype} "
+                         f"{list(t.shape)}")
+    return t
+
+
+def _cache(what, k, v, ks, vs, table, rows, dtype):
+    """Checks a cache's pages, scales and table -> (pages, Hk, page size, D, dtype code, the strides' and scales'
+    arguments of the C ABI)."""
+    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+        raise ValueError(f"{what}: the key and value pages must be [pages, kv heads, page size, D] alike, not "
+                         f"{list(k.shape)} and {list(v.shape)}")
+    N, Hk, ps, D = k.shape
+    if k.stride(3) != 1 and N and ps:
+        raise ValueError(f"{what}: the pages' last dimension must be contiguous")
+    fp8 = k.dtype == E4M3
+    if not fp8 and k.dtype != dtype:
+        raise ValueError(f"{what}: pages of {k.dtype} with tokens of {dtype}")
+    sp = sh = 0
+    if fp8:
+        if ks is None or vs is None or ks.shape != (N, Hk, ps) or vs.shape != ks.shape or ks.stride() != vs.stride() \
+                or ks.dtype != torch.float32 or vs.dtype != torch.float32 or (ps > 1 and ks.stride(2) != 1):
+            raise ValueError(f"{what}: 8-bit pages need fp32 scales k_scale, v_scale [{N}, {Hk}, {ps}]")
+        sp, sh, _ = ks.stride()
+    elif ks is not None or vs is not None:
+        raise ValueError(f"{what}: scales are for 8-bit pages")
+    _int32(f"{what}: the table", table, rows, None)
+    if table.shape[1] > 1 and table.stride(1) != 1:
+        raise ValueError(f"{what}: a table's rows must be contiguous")
+    return N, Hk, ps, D, _lib.E4M3 if fp8 else code(dtype), (*k.stride()[:3], ptr(ks), ptr(vs), sp, sh, N, ps,
+                                                             ptr(table), table.stride(0), table.shape[1])
+
+
+@_step_op("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, float scale, "
+          "int window=0, Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor",
+          lambda q, *a: q.new_empty(q.shape))
+def _paged_attention(q, k_pages, v_pages, table, lengths, scale, window=0, k_scale=None, v_scale=None):
+    require_cuda(q)
+    dev = q.device
+    _on(dev, k_pages, v_pages, table, lengths, k_scale, v_scale)
+    if q.dim() != 3:
+        raise ValueError(f"paged_attention: q must be [rows, heads, D], not {list(q.shape)}")
+    rows, H, D = q.shape
+    N, Hk, ps, Dk, kvt, cache = _cache("paged_attention", k_pages, v_pages, k_scale, v_scale, table, rows, q.dtype)
+    if D != Dk or H == 0 or H % Hk:
+        raise ValueError(f"paged_attention: {H} heads of {D} over pages of {Hk} heads of {Dk}")
+    _int32("paged_attention: lengths", lengths, rows)
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+    n = _lib.lib().basal200_paged_attention_workspace_bytes(rows, H, Hk, D, table.shape[1], ps, window)
+    work = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
+    call("basal200_paged_attention", dev, ptr(q), code(q.dtype), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages),
+         kvt, *cache, ptr(_c(lengths)), rows, H, Hk, D, scale, window, ptr(out), ptr(work), n)
+    return out
+
+
+def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
+                    window: int = 0, k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None) -> Tensor:
+    """Attention of one new token a row over a paged cache: q [rows, heads, D] (bf16 / fp16) -> [rows, heads, D], the
+    softmax over the row's positions max(0, length - window) <= t < length (window 0: all). k_pages, v_pages [pages,
+    kv heads, page size, D], D = 64, 128 or 256, of q's type, or e4m3 with fp32 k_scale, v_scale [pages, kv heads, page
+    size]; table [rows, width] int32: the page of positions j * page size ..; lengths [rows] int32, the new token's
+    own position included (its key and value are appended first). Heads share key / value heads in order. A length <= 0
+    gives zeros. A page that is needed and not there, or a length past the table, gives a NaN row and a fault bit.
+    Pages may be strided views (their last dimension contiguous, the others multiples of 16 bytes). A row's output is
+    the same bits alone and among other rows."""
+    return _paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)
+
+
+@_step_op("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, "
+          "Tensor? count=None, Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> ()")
+def _kv_append(k, v, k_pages, v_pages, table, start, count=None, k_scale=None, v_scale=None):
+    require_cuda(k)
+    dev = k.device
+    _on(dev, v, k_pages, v_pages, table, start, count, k_scale, v_scale)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"kv_append: k and v must be [rows, tokens, kv heads, D] alike, not {list(k.shape)} and "
+                         f"{list(v.shape)}")
+    rows, T, h, d = k.shape
+    N, Hk, ps, D, kvt, cache = _cache("kv_append", k_pages, v_pages, k_scale, v_scale, table, rows, k.dtype)
+    if (h, d) != (Hk, D):
+        raise ValueError(f"kv_append: tokens of {h} heads of {d} into pages of {Hk} heads of {D}")
+    _int32("kv_append: start", start, rows)
+    if count is not None:
+        count = _c(_int32("kv_append: count", count, rows))
+    k, v = (x if x.stride(3) == 1 and not (x.stride(0) | x.stride(1) | x.stride(2)) % 8 and not x.data_ptr() % 16
+            else x.contiguous() for x in (k, v))
+    (strides, scales), rest = (cache[:3], cache[3:7]), cache[7:]
+    call("basal200_kv_append", dev, ptr(k), ptr(v), code(k.dtype), *k.stride()[:3], *v.stride()[:3], ptr(k_pages),
+         ptr(v_pages), kvt, *strides, *scales, *rest, ptr(_c(start)), ptr(count), rows, T, Hk, D)
+
+
+def kv_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, start: Tensor,
+              count: Optional[Tensor] = None, k_scale: Optional[Tensor] = None,
+              v_scale: Optional[Tensor] = None) -> None:
+    """Writes new tokens into a paged cache: token t < count[b] (None: every one) of row b of k, v [rows, tokens, kv
+    heads, D] goes to position start[b] + t, through the table. start, count [rows] int32; start < 0: the row brings
+    nothing. Pages, scales and table as paged_attention's; e4m3 pages take fp8_act_quant's codes and scale of a token's
+    D values of a head. A position that no page of the cache holds is not written and sets a fault bit. Rows must not
+    share the pages that they write."""
+    _kv_append(k, v, k_pages, v_pages, table, start, count, k_scale, v_scale)
+
+
+@_step_op("kv_copy_pages(Tensor(a!)[] pools, int[] src, int[] dst) -> ()")
+def _kv_copy_pages(pools, src, dst):
+    if len(src) != len(dst):
+        raise ValueError(f"kv_copy_pages: {len(src)} pages to read, {len(dst)} to write")
+    require_cuda(*pools)
+    dev, N = pools[0].device, pools[0].shape[1] if pools[0].dim() > 1 else -1
+    _on(dev, *pools)
+    for p in pools:
+        if p.dim() < 3 or p.shape[1] != N or not p.is_contiguous():
+            raise ValueError("kv_copy_pages: the pools must be contiguous [layers, pages, ...] of equally many pages")
+    if any(not 0 <= i < N for i in src) or any(not 0 <= i < N for i in dst):
+        raise ValueError(f"kv_copy_pages: a page is outside [0, {N})")
+    n, m = len(src), len(pools)
+    if n == 0 or any(p.numel() == 0 for p in pools):
+        return
+    call("basal200_kv_copy_pages", dev, (ctypes.c_void_p * m)(*(p.data_ptr() for p in pools)),
+         (ctypes.c_int * m)(*(p.shape[0] for p in pools)),
+         (ctypes.c_int64 * m)(*(p.stride(1) * p.element_size() for p in pools)), m, N, (ctypes.c_int32 * n)(*src),
+         (ctypes.c_int32 * n)(*dst), n)
+
+
+def kv_copy_pages(pools: list[Tensor], src: list[int], dst: list[int]) -> None:
+    """Copies page src[i] over page dst[i] in every layer of every pool ([layers, pages, ...], contiguous; up to 8: a
+    cache's keys, values and their scales). src and dst are host lists, read before the call returns; ValueError, and
+    nothing copied, when a page is out of range, written twice, or both read and written."""
+    if pools:  # the dispatcher goes by a tensor
+        _kv_copy_pages(pools, src, dst)
+
+
+@_step_op("gdn_step(Tensor proj, Tensor(a!) tail, Tensor conv, Tensor A_log, Tensor dt_bias, Tensor(b!) state, int Hk, "
+          "int Hv, int b_off, int a_off, Tensor? slots=None) -> Tensor",
+          lambda proj, tail, conv, A_log, dt_bias, state, Hk, Hv, *a: proj.new_empty((proj.shape[0], Hv, 1, 128)))
+def _gdn_step(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots=None):
+    require_cuda(proj)
+    dev, dt = proj.device, proj.dtype
+    _on(dev, tail, conv, A_log, dt_bias, state, slots)
+    if proj.dim() != 2 or Hk <= 0 or Hv <= 0 or Hv % Hk:
+        raise ValueError(f"gdn_step: proj must be [rows, width], Hv a multiple of Hk, not {list(proj.shape)}, {Hv}, {Hk}")
+    rows, C = proj.shape[0], (2 * Hk + Hv) * 128
+    if state.dim() != 4 or state.shape[1:] != (Hv, 128, 128) or state.dtype != torch.float32 \
+            or not state.is_contiguous():
+        raise ValueError(f"gdn_step: the state must be contiguous fp32 [slots, {Hv}, 128, 128]")
+    if tail.shape != (state.shape[0], 3, C) or tail.dtype != dt or not tail.is_contiguous():
+        raise ValueError(f"gdn_step: the tail must be contiguous {dt} [{state.shape[0]}, 3, {C}]")
+    if conv.shape != (C, 4) or A_log.shape != (Hv,) or dt_bias.shape != (Hv,):
+        raise ValueError(f"gdn_step: conv must be [{C}, 4], A_log and dt_bias [{Hv}]")
+    if b_off < 0 or a_off < 0 or max(C, b_off + Hv, a_off + Hv) > proj.shape[1]:
+        raise ValueError(f"gdn_step: the projection has {proj.shape[1]} columns")
+    if slots is not None:
+        slots = _c(_int32("gdn_step: slots", slots, rows))
+    elif rows > state.shape[0]:
+        raise ValueError(f"gdn_step: {rows} rows, {state.shape[0]} states")
+    if proj.stride(1) != 1 or proj.stride(0) % 4 or proj.data_ptr() % 8:
+        proj = _aligned_rows(proj)
+    o = torch.empty((rows, Hv, 1, 128), dtype=dt, device=dev)
+    call("basal200_gdn_step", dev, ptr(proj), code(dt), proj.stride(0), ptr(tail), ptr(_c(conv.to(dt))),
+         ptr(_c(A_log.float())), ptr(_c(dt_bias.to(dt))), b_off, a_off, ptr(state), ptr(slots), state.shape[0], rows,
+         Hk, Hv, ptr(o))
+    return o
+
+
+def _aligned_rows(x):
+    """A copy of x [rows, width] whose rows start at multiples of 16 bytes."""
+    y = torch.empty((x.shape[0], x.shape[1] + -x.shape[1] % 8), dtype=x.dtype, device=x.device)[:, :x.shape[1]]
+    return y.copy_(x)
+
+
+def gdn_step(proj: Tensor, tail: Tensor, conv: Tensor, A_log: Tensor, dt_bias: Tensor, state: Tensor, Hk: int, Hv: int,
+             b_off: int, a_off: int, slots: Optional[Tensor] = None) -> Tensor:
+    """The Gated DeltaNet for one new token a row: gdn_prep's input steps and gdn_chunk_rule's recurrence for T = 1 in
+    one kernel. proj [rows, width] (bf16 / fp16; its q, k, v channels from column 0, b at b_off, a at a_off), the
+    convolution's last inputs tail [slots, 3, C] (oldest first) and the state [slots, Hv, 128, 128] fp32, both updated
+    in place -> o [rows, Hv, 1, 128] in proj's type. slots [rows] int32: each row's place in tail and state (None: its
+    number); negative: a row of padding, zeros, and nothing is updated. A slot that is not there, or that an earlier
+    row of the call has, gives a NaN row, no update and a fault bit."""
+    return _gdn_step(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots)
+
+
+@_step_op("constrain_logits(Tensor logits, Tensor? mask=None, Tensor? past=None, Tensor? repetition=None, "
+          "Tensor? presence=None, Tensor? frequency=None, Tensor? bias_ids=None, Tensor? bias_values=None) -> Tensor",
+          lambda logits, *a: logits.new_empty(logits.shape, dtype=torch.float32))
+def _constrain_logits(logits, mask=None, past=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                      bias_values=None):
+    require_cuda(logits)
+    dev = logits.device
+    _on(dev, mask, past, repetition, presence, frequency, bias_ids, bias_values)
+    if logits.dim() != 2:
+        raise ValueError(f"constrain_logits: logits must be [rows, vocabulary], not {list(logits.shape)}")
+    rows, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    rowwise = []
+    for what, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if t is not None and (t.shape != (rows,) or t.dtype != torch.float32):
+            raise ValueError(f"constrain_logits: {what} must be fp32 [{rows}], not {t.dtype} {list(t.shape)}")
+        rowwise.append(None if t is None else _c(t))
+    if past is None and any(t is not None for t in rowwise):
+        raise ValueError("constrain_logits: penalties need the rows' history (past)")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("constrain_logits: bias_ids and bias_values come together")
+    mrow = prow = brow = T = N = 0
+    if mask is not None:
+        _int32("constrain_logits: the mask", mask, None, -(-V // 32))
+        if mask.shape[0] not in (1, rows):
+            raise ValueError(f"constrain_logits: a mask of {mask.shape[0]} rows for {rows}")
+        mask = _c(mask)
+        mrow = mask.shape[1] if mask.shape[0] == rows else 0
+    if past is not None:
+        past = _c(_int32("constrain_logits: past", past, rows, None))
+        prow = T = past.shape[1]
+    if bias_ids is not None:
+        bias_ids = _c(_int32("constrain_logits: bias_ids", bias_ids, rows, None))
+        if bias_values.shape != bias_ids.shape or bias_values.dtype != torch.float32:
+            raise ValueError(f"constrain_logits: bias_values must be fp32 {list(bias_ids.shape)}")
+        bias_values = _c(bias_values)
+        brow = N = bias_ids.shape[1]
+    out = torch.empty((rows, V), dtype=torch.float32, device=dev)
+    call("basal200_constrain_logits", dev, ptr(logits), code(logits.dtype), logits.stride(0), rows, V, ptr(mask), mrow,
+         ptr(past), prow, T, *map(ptr, rowwise), ptr(bias_ids), ptr(bias_values), brow, N, ptr(out))
+    return out
+
+
+def constrain_logits(logits: Tensor, mask: Optional[Tensor] = None, past: Optional[Tensor] = None,
+                     repetition: Optional[Tensor] = None, presence: Optional[Tensor] = None,
+                     frequency: Optional[Tensor] = None, bias_ids: Optional[Tensor] = None,
+                     bias_values: Optional[Tensor] = None) -> Tensor:
+    """A step's logits [rows, V] (bf16 / fp16 / fp32) under penalties, biases and a grammar mask -> fp32 [rows, V]:
+    a token that occurs n > 0 times in past [rows, T] (int32, negative entries skipped) gets z = (z > 0 ? z /
+    repetition : z * repetition) - (frequency * n + presence), each fp32 [rows]; then the values listed for it in
+    bias_ids (int32) / bias_values (fp32) [rows, N], N <= 4096, are added, in the list's order; then the tokens whose
+    bit v % 32 of word v / 32 of mask [rows or 1, ceil(V / 32)] (int32) is 0 become -inf, whatever their logit (a row
+    with no bit set is all -inf). Token ids >= V are skipped and set a fault bit."""
+    return _constrain_logits(logits, mask, past, repetition, presence, frequency, bias_ids, bias_values)

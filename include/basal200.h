@@ -29,8 +29,8 @@ enum {
   BASAL200_ERR_LIMIT = 8    /* a size beyond what the entry point was built for */
 };
 
-/* Element type codes of activations, outputs and biases. */
-enum { BASAL200_BF16 = 0, BASAL200_F16 = 1, BASAL200_F32 = 2 };
+/* Element type codes of activations, outputs and biases; E4M3 only for the pages of a key / value cache. */
+enum { BASAL200_BF16 = 0, BASAL200_F16 = 1, BASAL200_F32 = 2, BASAL200_E4M3 = 3 };
 
 /* ---- FP8-block / INT8-block (128 x 128 weight blocks, 1 x 128 activation groups, fp32 scales) ---- */
 
@@ -295,17 +295,89 @@ int basal200_code_probs(const float* z, int64_t R, int64_t U, const int64_t* idx
                         float* p, void* stream);
 
 
+/* ---- One new token a row: the paged key / value cache, the recurrent state, the next token's logits ----
+ *
+ * The reference answers from one prefill pass and has none of these. A cache's keys and its values are two pools of
+ * pages [pages, Hk, page_size, D] (element strides page_stride, head_stride, token_stride, the same for both; D
+ * contiguous; 16-byte aligned rows), D = 64, 128 or 256, bf16, fp16 or e4m3. e4m3 pools have fp32 scales ks / vs
+ * [pages, Hk, page_size] (strides s_page, s_head; tokens contiguous): a value is code * scale. Position t of row b is
+ * at offset t % page_size of page table[b * table_row + t / page_size] (width entries a row). A table entry is read
+ * only for a position that the call reads or writes; one outside [0, pages) is never followed: the fault bit
+ * BASAL200_FAULT_BAD_PAGE is set, an attention row that needs it is NaN, a new token that needs it is not written. */
+
+/* out [rows, H, D] (q_dtype bf16 or fp16, contiguous) = softmax(scale q . k_t) v over each row's positions
+ * max(0, lengths[b] - window) <= t < lengths[b] (window 0: from 0). q [rows, H, D] with element strides q_row, q_head;
+ * head h reads key / value head h / (H / Hk). A length <= 0 gives zeros; one above width * page_size gives NaN and
+ * the fault bit. 16-bit pools have q's type. A row's bits do not depend on the other rows of the call. workspace
+ * (16-byte aligned): basal200_paged_attention_workspace_bytes(...) bytes. */
+int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t q_head, const void* k, const void* v,
+                             int kv_dtype, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                             const float* ks, const float* vs, int64_t s_page, int64_t s_head, int64_t pages,
+                             int page_size, const int32_t* table, int64_t table_row, int width,
+                             const int32_t* lengths, int rows, int H, int Hk, int D, float scale, int window,
+                             void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of basal200_paged_attention for rows of up to width * page_size positions; 0: none is needed (NULL
+ * allowed). Pure: no device call. */
+int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int width, int page_size, int window);
+
+/* Writes tokens t < min(T, count[b]) (count NULL: T) of row b's new keys and values (k, v [rows, T, Hk, D], dtype bf16
+ * or fp16, element strides k_row, k_tok, k_head and v_...; D contiguous, 16-byte aligned) into the pools at positions
+ * start[b] + t. start[b] < 0: the row brings nothing. 16-bit pools have the tokens' type and take their bits; e4m3
+ * pools take codes and scales by basal200_fp8_act_quant's arithmetic over a token's D values of a head (scale =
+ * max(amax, 1e-12) / 448; a NaN makes the scale NaN). Rows must not share pages that they write. */
+int basal200_kv_append(const void* k, const void* v, int dtype, int64_t k_row, int64_t k_tok, int64_t k_head,
+                       int64_t v_row, int64_t v_tok, int64_t v_head, void* k_pool, void* v_pool, int kv_dtype,
+                       int64_t page_stride, int64_t head_stride, int64_t token_stride, float* ks, float* vs,
+                       int64_t s_page, int64_t s_head, int64_t pages, int page_size, const int32_t* table,
+                       int64_t table_row, int width, const int32_t* start, const int32_t* count, int rows, int T,
+                       int Hk, int D, void* stream);
+
+/* Copies page src[i] over page dst[i], i < n, in every layer of each of npools <= 8 pools: pools[j] holds layers[j]
+ * layers of `pages` pages of page_bytes[j] bytes each, contiguous; 4-byte aligned, page_bytes a multiple of 4.
+ * pools, layers, page_bytes, src and dst are host arrays, read before the call returns. BASAL200_ERR_ARG, and nothing
+ * copied, when an index is outside [0, pages), a page is written twice, or a page is both read and written. */
+int basal200_kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_bytes, int npools,
+                           int64_t pages, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* One token of the Gated DeltaNet for each row: basal200_gdn_prep's input steps for T = 1 (the same roundings) and
+ * basal200_gdn_chunk_rule's recurrence, with the row's last 3 convolution inputs tail [slots, 3, C] (16-bit, oldest
+ * first, C = (2 Hk + Hv) * 128) and state [slots, Hv, 128, 128] (fp32) updated in place -> o [rows, Hv, 128] in
+ * dtype. proj, conv, A_log, dt_bias, b_off, a_off as basal200_gdn_prep's. at [rows] is each row's slot (NULL: its
+ * number); a negative one is a row of padding: zeros, and nothing is updated. A slot >= slots, or one that an earlier
+ * row of the call has, is refused: the row's output is NaN, nothing of it is updated, and the fault bit
+ * BASAL200_FAULT_BAD_SLOT is set. */
+int basal200_gdn_step(const void* proj, int dtype, int64_t ld, void* tail, const void* conv, const float* A_log,
+                      const void* dt_bias, int b_off, int a_off, float* state, const int32_t* at, int64_t slots,
+                      int rows, int Hk, int Hv, void* o, void* stream);
+
+/* out [rows, V] fp32 from logits [rows, V] (dtype bf16, fp16 or fp32, row stride ld): for a token that occurs n > 0
+ * times in the row's history past [rows, T] (row stride past_row), z = (z > 0 ? z / repetition[b] : z *
+ * repetition[b]) - (frequency[b] * n + presence[b]); then the values listed for it in ids / values [rows, N] (row
+ * stride bias_row; added in the list's order where it is listed more than once) are added; then -inf where bit v % 32
+ * of word v / 32 of mask [rows, ceil(V / 32)] (row stride mask_row, 0: one row for all) is 0, whatever the logit.
+ * Negative ids in past and ids are skipped; one >= V is skipped and sets BASAL200_FAULT_BAD_ID. mask, past, ids,
+ * repetition, presence and frequency may be NULL (no mask, T = 0, N = 0, 1, 0, 0). */
+int basal200_constrain_logits(const void* logits, int dtype, int64_t ld, int rows, int V, const uint32_t* mask,
+                              int64_t mask_row, const int32_t* past, int64_t past_row, int T,
+                              const float* repetition, const float* presence, const float* frequency,
+                              const int32_t* ids, const float* values, int64_t bias_row, int N, float* out,
+                              void* stream);
+
 /* ---- Diagnostics ---- */
 
 /* Fault bits (basal200_device_faults): a bounded wait of a GEMM gave up (producer, MMA issuer, epilogue, drain), a
- * readout id was out of range, or a peer barrier's wait for another rank gave up. */
+ * readout id or a token id was out of range, a peer barrier's wait for another rank gave up, a cache's table named a
+ * page that is not there (or a row was longer than its table), or a row's state slot was out of range or taken. */
 enum {
   BASAL200_FAULT_TIMEOUT_PRODUCER = 1,
   BASAL200_FAULT_TIMEOUT_MMA = 2,
   BASAL200_FAULT_TIMEOUT_EPILOGUE = 4,
   BASAL200_FAULT_TIMEOUT_DRAIN = 8,
   BASAL200_FAULT_BAD_ID = 16,
-  BASAL200_FAULT_TIMEOUT_PEER = 32
+  BASAL200_FAULT_TIMEOUT_PEER = 32,
+  BASAL200_FAULT_BAD_PAGE = 64,
+  BASAL200_FAULT_BAD_SLOT = 128
 };
 
 /* The fault bits kernels on `device` recorded when a bounded wait gave up (0: none); clear != 0 resets them.

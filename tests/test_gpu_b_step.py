@@ -1,0 +1,437 @@
+"""One new token a row on the GPU: basal::gdn_step, basal::constrain_logits, the paged cache's bookkeeping over real
+pages, and the hybrid classifier carried token by token.
+
+gdn_step against the recurrence in 64 bits from operands in torch's 32-bit statement of the input steps (which the
+kernel's convolution and gates equal bit for bit, its q and k to 2^-21). Tolerances, per value: a sum of 128 products in
+32 bits is off by at most 136 * 2^-24 of the sum of magnitudes, and the operands' errors stay under 24 * 2^-24 more, so
+with A = decay |S| + |k| (|v| + sum_i |k_i S_i|) the state is off by at most 160 * 2^-24 A, and the output by its own
+rounding (eps / 2) and 160 * 2^-24 sum_i |q_i| (A_i + |S'_i|).
+constrain_logits against the definition in 64 bits: at most 4 roundings of 2^-24 of the magnitudes that it adds.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_9_hybrid import torch_prep
+
+pytestmark = pytest.mark.gpu
+BF, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from basal_b200 import _lib, ops
+    _lib.device_faults(0)
+    yield ops
+    assert _lib.device_faults(0) == 0
+
+
+def faults():
+    from basal_b200 import _lib
+    return _lib.device_faults(0)
+
+
+def inputs(rows, slots, Hk, Hv, dtype, seed=0, pad=64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    C = (2 * Hk + Hv) * 128
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    return dict(proj=r(rows, C + Hv * 128 + 2 * Hv + pad).to(dtype), tail=r(slots, 3, C).to(dtype),
+                conv=(torch.rand(C, 4, device="cuda", generator=g) - 0.5).to(dtype),
+                A_log=torch.log(1 + 15 * torch.rand(Hv, device="cuda", generator=g)),
+                dt_bias=(1 + 0.1 * r(Hv)).to(dtype), state=r(slots, Hv, 128, 128) * 0.3, Hk=Hk, Hv=Hv,
+                b_off=C + Hv * 128, a_off=C + Hv * 128 + Hv)
+
+
+def reference(x, slots):
+    """(o, tol_o, state, tol_state, tail) of the rows with a slot, in 64 bits."""
+    live = [b for b, s in enumerate(slots) if s >= 0]
+    at = torch.tensor([slots[b] for b in live], device="cuda")
+    proj, tail, Hk, Hv = x["proj"][live], x["tail"][at], x["Hk"], x["Hv"]
+    q, k, v, beta, g = torch_prep(proj, tail, x["conv"], x["A_log"], x["dt_bias"], len(live), 1, Hk, Hv, x["b_off"],
+                                  x["a_off"])
+    q, k, v = (t[:, :, 0].double() for t in (q, k, v))
+    beta, decay = beta[:, :, 0].double()[..., None], g[:, :, 0].double().exp()[..., None, None]
+    S = x["state"][at].double() * decay
+    kv = (S * k[..., None]).sum(2)
+    big = S.abs() + k.abs()[..., None] * (v.abs() + (S * k[..., None]).abs().sum(2))[:, :, None]
+    S = S + k[..., None] * (beta * (v - kv))[:, :, None]
+    o = (S * q[..., None]).sum(2)
+    unit = 160 * 2.0 ** -24
+    fi = torch.finfo(x["proj"].dtype)
+    # a value below the type's smallest normal one is rounded to a multiple of tiny * eps: off by half of that
+    tol_o = fi.eps / 2 * o.abs().clamp(min=fi.tiny) + unit * (q.abs()[..., None] * (big + S.abs())).sum(2)
+    new_tail = torch.cat([tail[:, 1:], proj[:, None, :tail.shape[2]]], 1)
+    return live, at, o, tol_o, S, unit * big, new_tail
+
+
+def step(ops, x, slots=None):
+    return ops.gdn_step(x["proj"], x["tail"], x["conv"], x["A_log"], x["dt_bias"], x["state"], x["Hk"], x["Hv"],
+                        x["b_off"], x["a_off"], slots)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("rows, spare, Hk, Hv", [(1, 0, 16, 32), (3, 4, 1, 1), (5, 2, 2, 6), (2, 0, 4, 4), (40, 7, 1, 3),
+                                                 (2, 1, 1, 8)])
+def test_gdn_step(ops, dtype, rows, spare, Hk, Hv):
+    x = inputs(rows, rows + spare, Hk, Hv, dtype, seed=rows)
+    order = torch.randperm(rows + spare, generator=torch.Generator().manual_seed(rows)).tolist()[:rows]
+    if rows > 2:
+        order[1] = -1
+    if rows > 4:
+        order[-1] = -7
+    live, at, o, tol_o, S, tol_S, tail = reference(x, order)
+    state0, tail0 = x["state"].clone(), x["tail"].clone()
+    got = step(ops, x, torch.tensor(order, dtype=torch.int32, device="cuda"))
+    assert got.shape == (rows, Hv, 1, 128) and got.dtype == dtype
+    assert ((got[live, :, 0].double() - o).abs() <= tol_o).all()
+    assert ((x["state"][at].double() - S).abs() <= tol_S).all()
+    assert torch.equal(x["tail"][at], tail)
+    rest = torch.ones(rows + spare, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert torch.equal(x["state"][rest], state0[rest]) and torch.equal(x["tail"][rest], tail0[rest])
+    for b in set(range(rows)) - set(live):
+        assert not got[b].any()
+
+
+def test_gdn_step_continues_the_chunk_rule(ops):
+    """A prompt by chunks and 5 tokens one by one, against the whole sequence by chunks: within the chunk rule's own
+    bar (1e-4 of the per-token definition) for state and 16-bit outputs' rounding."""
+    rows, T, Hk, Hv = 3, 75, 2, 4
+    x = inputs(rows * T, rows, Hk, Hv, BF, seed=1)
+    proj = x["proj"].view(rows, T, -1)
+    zero = torch.zeros(rows, 3, x["tail"].shape[2], dtype=BF, device="cuda")
+
+    def chunk(p, n):
+        q, k, v, beta, g = ops.gdn_prep(p.reshape(rows * n, -1), zero, x["conv"], x["A_log"], x["dt_bias"], rows, n, Hk,
+                                        Hv, x["b_off"], x["a_off"])
+        return ops.gdn_chunk_rule(q, k, v, g, beta, None, True)
+
+    o, s = chunk(proj, T)
+    _, x["state"] = chunk(proj[:, :T - 5], T - 5)
+    x["tail"] = proj[:, T - 8:T - 5, :x["tail"].shape[2]].contiguous()
+    for t in range(T - 5, T):
+        x["proj"] = proj[:, t]
+        got = step(ops, x)
+        want = o[:, :, t].float()
+        assert ((got[:, :, 0].float() - want).abs() <= 2.0 ** -7 * want.abs() + 1e-4).all()
+    assert (x["state"] - s).abs().max() <= 1e-4
+    assert torch.equal(x["tail"], proj[:, T - 3:, :x["tail"].shape[2]])
+
+
+def test_gdn_step_row_alone_and_among_others(ops):
+    a, b = (inputs(70, 70, 4, 8, BF, seed=2) for _ in range(2))
+    whole = step(ops, a)
+    for r in (0, 33, 69):
+        one = {**b, "proj": b["proj"][r:r + 1]}
+        got = step(ops, one, torch.tensor([r], dtype=torch.int32, device="cuda"))
+        assert torch.equal(got[0], whole[r]) and torch.equal(b["state"][r], a["state"][r])
+
+
+def test_gdn_step_strided_projection(ops):
+    a, b, c = (inputs(6, 6, 2, 2, BF, seed=3) for _ in range(3))
+    want = step(ops, a)
+    wide = torch.zeros(6, b["proj"].shape[1] + 8, dtype=BF, device="cuda")
+    wide[:, :-8] = b["proj"]
+    assert torch.equal(step(ops, {**b, "proj": wide[:, :-8]}), want)
+    odd = torch.zeros(6, c["proj"].shape[1] + 9, dtype=BF, device="cuda")
+    odd[:, 3:-6] = c["proj"]
+    assert torch.equal(step(ops, {**c, "proj": odd[:, 3:-6]}), want) and torch.equal(c["state"], a["state"])
+
+
+def test_gdn_step_refused_slots(ops):
+    """A slot that is not there or taken by an earlier row: NaN, the fault bit, and nothing of it is updated."""
+    x = inputs(5, 4, 2, 4, BF, seed=4)
+    y = {k: v.clone() if torch.is_tensor(v) else v for k, v in x.items()}
+    got = step(ops, x, torch.tensor([2, 4, 2, 0, -1], dtype=torch.int32, device="cuda"))
+    assert faults() == 128
+    want = step(ops, {**y, "proj": y["proj"][[0, 3]]}, torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got[[0, 3]], want) and got[1:3].isnan().all() and not got[4].any()
+    assert torch.equal(x["state"], y["state"]) and torch.equal(x["tail"], y["tail"])
+
+
+def test_gdn_step_captured(ops):
+    x = inputs(2, 2, 4, 8, BF, seed=5)
+    y = {k: v.clone() if torch.is_tensor(v) else v for k, v in x.items()}
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = step(ops, x)
+    for _ in range(3):
+        g.replay()
+        want = step(ops, y)
+        assert torch.equal(o, want) and torch.equal(x["state"], y["state"]) and torch.equal(x["tail"], y["tail"])
+
+
+def test_gdn_step_refusals(ops):
+    x = inputs(3, 3, 2, 4, BF, seed=6)
+    def no(**kw):
+        with pytest.raises(ValueError):
+            step(ops, {**x, **{k: v for k, v in kw.items() if k != "slots"}}, kw.get("slots"))
+    no(Hk=3)
+    no(proj=x["proj"].float())
+    no(state=x["state"].bfloat16())
+    no(state=x["state"].transpose(2, 3))
+    no(state=x["state"][:2], tail=x["tail"][:2])          # fewer states than rows, and no slots
+    no(tail=x["tail"][:, :2])
+    no(tail=x["tail"].half())
+    no(conv=x["conv"][:, :3])
+    no(b_off=x["proj"].shape[1] - 3)
+    no(slots=torch.zeros(3, dtype=torch.int64, device="cuda"))
+    no(slots=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    no(state=x["state"].cpu())
+    assert step(ops, {**x, "proj": x["proj"][:0]}).shape == (0, 4, 1, 128)
+
+
+# --- logits ------------------------------------------------------------------------------------------------------
+def wanted(z, mask, past, rep, pres, freq, ids, vals):
+    """The definition in 64 bits, and the sum of the magnitudes that were added."""
+    rows, V = z.shape
+    z = z.double()
+    size = z.abs().nan_to_num(0, 0, 0)
+    for r in range(rows):
+        if past is not None:
+            h = past[r][past[r] >= 0].long()
+            n = torch.bincount(h[h < V], minlength=V).double()
+            rr = 1.0 if rep is None else rep[r].double()
+            f, p = (0.0 if t is None else t[r].double() for t in (freq, pres))
+            hit = n > 0
+            x = torch.where(z[r] > 0, z[r] / rr, z[r] * rr)
+            z[r] = torch.where(hit, x - (f * n + p), z[r])
+            size[r] = torch.where(hit, torch.maximum(size[r], x.abs().nan_to_num(0, 0, 0)) + (f * n + p), size[r])
+        if ids is not None:
+            for i, x in zip(ids[r].tolist(), vals[r].tolist()):
+                if 0 <= i < V:
+                    z[r, i] += x
+                    size[r, i] += abs(x)
+    if mask is not None:
+        bits = (mask[:, :, None] >> torch.arange(32, device="cuda") & 1).flatten(1)[:, :V].expand(rows, V)
+        z = torch.where(bits != 0, z, -math.inf)
+    return z, size
+
+
+def compare(got, want, size):
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got)) and torch.equal(got.isnan(), want.isnan())
+    rest = ~fine & ~want.isnan()
+    assert torch.equal(got[rest].double(), want[rest])
+    assert ((got.double() - want).abs()[fine] <= 4 * 2.0 ** -24 * size[fine]).all()
+
+
+def words(rows, V, share, g):
+    bits = torch.rand(rows, -(-V // 32) * 32, device="cuda", generator=g) < share
+    w = (bits.view(rows, -1, 32).long() << torch.arange(32, device="cuda")).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16, torch.float32])
+@pytest.mark.parametrize("rows, V, T, N, share", [(1, 1, 1, 1, 1.0), (3, 31, 5, 2, 0.5), (2, 32, 0, 3, 0.0),
+                                                  (4, 33, 9, 0, 0.9), (2, 2048, 300, 40, 0.3), (3, 2049, 700, 5, 0.01),
+                                                  (5, 32003, 4000, 300, 0.5), (2, 151936, 2000, 64, 0.001)])
+def test_constrain(ops, dtype, rows, V, T, N, share):
+    g = torch.Generator(device="cuda").manual_seed(V + T)
+    z = (torch.randn(rows, V, device="cuda", generator=g) * 4).to(dtype)
+    z[:, ::7] = 0
+    past = (torch.rand(rows, T, device="cuda", generator=g) ** 3 * V).to(torch.int32).clamp(max=V - 1)
+    past[:, ::5] = -1
+    ids = torch.randint(-1, V, (rows, N), device="cuda", generator=g, dtype=torch.int32)
+    vals = torch.randn(rows, N, device="cuda", generator=g)
+    if N > 3:
+        ids[:, 3] = ids[:, 1]  # one token listed twice
+    rep, pres, freq = (torch.rand(rows, device="cuda", generator=g) * s + o for s, o in ((0.5, 0.8), (1, 0), (0.3, 0)))
+    mask = words(rows, V, share, g)
+    if rows > 1:
+        mask[1] = 0  # a row whose mask leaves nothing
+    args = (mask, past, rep, pres, freq, ids, vals)
+    compare(ops.constrain_logits(z, *args), *wanted(z, *args))
+    compare(ops.constrain_logits(z), *wanted(z, None, None, None, None, None, None, None))
+    one = words(1, V, share, g)  # one mask for every row, alone
+    compare(ops.constrain_logits(z, one), *wanted(z, one, None, None, None, None, None, None))
+    compare(ops.constrain_logits(z, None, past, None, pres), *wanted(z, None, past, None, pres, None, None, None))
+    compare(ops.constrain_logits(z, None, past, rep), *wanted(z, None, past, rep, None, None, None, None))
+    compare(ops.constrain_logits(z, bias_ids=ids, bias_values=vals),
+            *wanted(z, None, None, None, None, None, ids, vals))
+
+
+def test_constrain_infinities_and_nans(ops):
+    z = torch.tensor([[float("nan"), float("inf"), -float("inf"), 1.0] * 9], device="cuda")
+    past = torch.tensor([[0, 1, 2, 3]], dtype=torch.int32, device="cuda")
+    rep = torch.tensor([2.0], device="cuda")
+    mask = torch.tensor([[0xFF0, 0xF]], dtype=torch.int32, device="cuda")
+    got = ops.constrain_logits(z, mask, past, rep)
+    want, size = wanted(z, mask, past, rep, None, None, None, None)
+    compare(got, want, size)
+    assert (got[0, :4] == -math.inf).all() and got[0, 4].isnan() and got[0, 5] == math.inf
+
+
+def test_constrain_strided_and_unaligned_logits(ops):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for dtype in (BF, torch.float32):
+        wide = torch.randn(4, 3001, device="cuda", generator=g).to(dtype)
+        for z in (wide[:, :2900], wide[:, 5:2905], wide[::2, 1:], wide.t()):
+            past = torch.randint(0, z.shape[1], (z.shape[0], 20), device="cuda", generator=g, dtype=torch.int32)
+            rep = torch.full((z.shape[0],), 1.3, device="cuda")
+            compare(ops.constrain_logits(z, None, past, rep), *wanted(z, None, past, rep, None, None, None, None))
+
+
+def test_constrain_ids_out_of_range(ops):
+    z = torch.zeros(1, 40, device="cuda")
+    bad = torch.tensor([[40, 3]], dtype=torch.int32, device="cuda")
+    got = ops.constrain_logits(z, None, bad, None, torch.ones(1, device="cuda"))
+    assert faults() == 16 and got[0, 3] == -1 and got.sum() == -1
+    got = ops.constrain_logits(z, bias_ids=bad, bias_values=torch.ones(1, 2, device="cuda"))
+    assert faults() == 16 and got[0, 3] == 1 and got.sum() == 1
+
+
+def test_constrain_captured(ops):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    z = torch.randn(2, 5000, device="cuda", generator=g).to(BF)
+    past = torch.full((2, 8), -1, dtype=torch.int32, device="cuda")
+    pres = torch.ones(2, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.constrain_logits(z, None, past, None, pres)
+    past[:, 0] = 17
+    z.neg_()
+    graph.replay()
+    compare(got, *wanted(z, None, past, None, pres, None, None, None))
+
+
+def test_constrain_refusals(ops):
+    z = torch.zeros(2, 40, device="cuda")
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    def no(*a, **kw):
+        with pytest.raises(ValueError):
+            ops.constrain_logits(*a, **kw)
+    no(z[0])
+    no(z.long())
+    no(z, i32(2, 1))                     # a mask of 32 tokens for 40
+    no(z, i32(3, 2))
+    no(z, i32(2, 2).long())
+    no(z, None, i32(1, 4))
+    no(z, None, None, torch.ones(2, device="cuda"))      # a penalty without a history
+    no(z, None, i32(2, 4), torch.ones(1, device="cuda"))
+    no(z, None, i32(2, 4), torch.ones(2, device="cuda").half())
+    no(z, bias_ids=i32(2, 4))
+    no(z, bias_ids=i32(2, 4), bias_values=torch.zeros(2, 3, device="cuda"))
+    no(z, bias_ids=i32(2, 5000), bias_values=torch.zeros(2, 5000, device="cuda"))
+    no(z.cpu())
+    assert ops.constrain_logits(z[:0]).shape == (0, 40)
+
+
+# --- the cache and the model --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cache_forks_grows_and_compacts(ops, fp8):
+    """Sequences of two layers through forks, copies before writing, freed and moved pages: what each attends to stays
+    what was appended to it (its keys and values rebuilt from the appended ones give the same bits)."""
+    from basal_b200.kvcache import PagedKVCache
+    g = torch.Generator(device="cuda").manual_seed(7)
+    Hk, D, L = 2, 64, 2
+    cache = PagedKVCache(L, 24, Hk, D, 16, BF, fp8)
+    said = {}
+
+    def put(seqs, n):
+        cache.grow(seqs, n)
+        b = cache.batch(seqs)
+        for layer in range(L):
+            k, v = (torch.randn(len(seqs), n, Hk, D, device="cuda", generator=g).to(BF) for _ in range(2))
+            cache.append(layer, b, k, v)
+            for i, s in enumerate(seqs):
+                said.setdefault((s, layer), []).append((k[i], v[i]))
+
+    def look(seqs):
+        b = cache.batch(seqs)
+        q = torch.randn(len(seqs), 4, D, device="cuda", generator=g).to(BF)
+        for layer in range(L):
+            got = cache.attend(layer, b, q, 0.125)
+            for i, s in enumerate(seqs):
+                fresh = PagedKVCache(1, 24, Hk, D, 16, BF, fp8)
+                one = fresh.add()
+                k, v = (torch.cat([x[j] for x in said[s, layer]])[None] for j in (0, 1))
+                fresh.grow([one], k.shape[1])
+                fb = fresh.batch([one])
+                fresh.append(0, fb, k, v)
+                assert torch.equal(fresh.attend(0, fb, q[i:i + 1], 0.125)[0], got[i]), (s, layer)
+
+    a = cache.add()
+    put([a], 37)
+    b, c = cache.fork(a), cache.fork(a)
+    for s in (b, c):
+        for layer in range(L):
+            said[s, layer] = list(said[a, layer])
+    assert cache.pages_of(a) == cache.pages_of(b) and cache.free_pages == 21
+    put([a, b], 1)          # two copies of the shared last page: c keeps the old one
+    put([c], 30)
+    look([a, b, c])
+    assert cache.pages_of(a)[:2] == cache.pages_of(b)[:2] == cache.pages_of(c)[:2]
+    assert len({cache.pages_of(s)[2] for s in (a, b, c)}) == 3
+    cache.free(b)
+    put([a], 40)
+    look([c, a])
+    n = cache.compact()
+    assert n == 24 - cache.free_pages and all(p < n for s in (a, c) for p in cache.pages_of(s))
+    look([a, c])
+    put([a, c], 3)
+    look([a, c])
+    with pytest.raises(MemoryError):
+        cache.grow([a], 16 * 24)
+    look([a, c])
+
+
+@pytest.mark.parametrize("fp8", [False])
+def test_model_token_by_token(ops, fp8):
+    """A small hybrid: 6 tokens one at a time after a suffix pass, against one suffix pass over all of them. Every
+    8-bit activation quantiser may move a code by one e4m3 step where two roundings differ, so the hidden states
+    agree to that step (2^-4 of a row's norm), the bar of the model's other tests."""
+    from basal_b200 import hybrid as hy
+    cfg = hy.HybridConfig(layers=4, hidden=512, heads=8, kv_heads=2, inter=512, vocab=1000, lin_k_heads=2, lin_v_heads=4)
+    m = hy.HybridClassifier(cfg, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    st = m.prefix(torch.randint(0, 1000, (100,), device="cuda", generator=g))
+    ids = torch.randint(0, 1000, (3, 46), device="cuda", generator=g)
+    want = [m.suffix_hidden(ids[:, :n], st).float() for n in range(40, 47)]
+    s = m.open(ids[:, :40], st, 6, page_size=16, fp8=fp8)
+    got = [s.hidden.float()] + [m.step(ids[:, t], s).float() for t in range(40, 46)]
+    assert s.position == 146 and all(s.cache.length(q) == 146 for q in s.seqs)
+    assert torch.equal(got[0], want[0])
+    for a, b in zip(got, want):
+        assert ((a - b).norm(dim=1) <= 2.0 ** -4 * b.norm(dim=1)).all()
+    with pytest.raises(MemoryError):
+        for t in range(20):
+            m.step(ids[:, 0], s)
+
+
+def test_model_answers_under_a_grammar(ops):
+    """Greedy answers: every token allowed by its step's mask, no token twice under a large presence penalty, and the
+    first token the unconstrained argmax where the mask leaves it."""
+    import torch.nn.functional as F
+    from basal_b200 import hybrid as hy
+    cfg = hy.HybridConfig(layers=4, hidden=256, heads=4, kv_heads=2, inter=256, vocab=777, lin_k_heads=1, lin_v_heads=2)
+    m = hy.HybridClassifier(cfg, seed=4)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    st = m.prefix(torch.randint(0, 777, (33,), device="cuda", generator=g))
+    ids = torch.randint(0, 777, (2, 20), device="cuda", generator=g)
+    free = m.answer(ids, st, 5)
+    top = F.linear(m.suffix_hidden(ids, st), m.head.weight).float().argmax(-1)
+    assert free.shape == (2, 5) and torch.equal(free[:, 0], top)
+    assert torch.equal(m.answer(ids, st, 5, fp8=True)[:, 0], top)
+    penal = torch.full((2,), 1e6, device="cuda")
+    seen = []
+
+    def grammar(past):
+        seen.append(past.shape[1])
+        mask = torch.zeros(1, 25, dtype=torch.int32, device="cuda")
+        mask[0, 3 + past.shape[1]] = 0x0F0F
+        mask[0, 0] = 6
+        return mask
+
+    got = m.answer(ids, st, 4, mask=grammar, presence=penal)
+    assert seen == [0, 1, 2, 3]
+    for row in got.tolist():
+        assert len(set(row)) == 4
+        for t, v in enumerate(row):
+            assert v in (1, 2) or (v // 32 == 3 + t and 0x0F0F >> v % 32 & 1)
+    assert m.answer(ids, st, 0).shape == (2, 0)

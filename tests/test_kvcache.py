@@ -1,0 +1,134 @@
+"""The paged cache's bookkeeping without a GPU: which page each sequence holds through growth, forks, frees and
+compaction, with the page copies recorded instead of run."""
+import pytest
+import torch
+
+from basal_b200 import kvcache
+
+
+@pytest.fixture
+def moved(monkeypatch):
+    got = []
+    monkeypatch.setattr(kvcache.ops, "kv_copy_pages", lambda pools, src, dst: got.append((list(src), list(dst))))
+    return got
+
+
+def cache(pages=10, page_size=4, **kw):
+    return kvcache.PagedKVCache(1, pages, 1, 64, page_size, device="cpu", **kw)
+
+
+def consistent(c):
+    held = {}
+    for s, pages in c._of.items():
+        assert len(pages) * c.page_size >= c.length(s) and len(set(pages)) == len(pages)
+        for p in pages:
+            held[p] = held.get(p, 0) + 1
+    assert [held.get(p, 0) for p in range(c.pages)] == c._shares
+    assert sorted(c._free) == [p for p in range(c.pages) if p not in held]
+
+
+def test_grow_and_free(moved):
+    c = cache()
+    a, b = c.add(), c.add()
+    c.grow([a, b], [4, 5])
+    assert [len(c.pages_of(s)) for s in (a, b)] == [1, 2] and c.free_pages == 7
+    c.grow([a])
+    assert len(c.pages_of(a)) == 2 and c.length(a) == 5
+    c.grow([a, b], 0)
+    consistent(c)
+    c.free(a)
+    assert c.free_pages == 8 and not moved
+    consistent(c)
+    with pytest.raises(KeyError):
+        c.grow([a])
+    with pytest.raises(KeyError):
+        c.fork(a)
+
+
+def test_fork_copies_only_what_is_written(moved):
+    c = cache()
+    a = c.add()
+    c.grow([a], 6)
+    full, half = c.pages_of(a)
+    b, d = c.fork(a), c.fork(a)
+    assert c.free_pages == 8
+    c.grow([a, b, d])  # three write the half-full page: two copies, the last keeps it
+    assert moved == [([half, half], [c.pages_of(a)[1], c.pages_of(b)[1]])]
+    assert c.pages_of(d) == [full, half] and c.pages_of(a)[0] == c.pages_of(b)[0] == full
+    consistent(c)
+    moved.clear()
+    c.grow([a, b, d], 1)  # nobody shares what is written now
+    assert not moved
+    e = c.fork(a)  # at a page's end (8 tokens of 4): nothing to copy, a new page each
+    c.grow([e, a])
+    assert not moved and c.pages_of(e)[:2] == c.pages_of(a)[:2] and c.pages_of(e)[2] != c.pages_of(a)[2]
+    consistent(c)
+
+
+def test_a_shared_page_is_copied_when_one_of_its_holders_writes(moved):
+    c = cache()
+    a = c.add()
+    c.grow([a], 2)
+    b = c.fork(a)
+    c.grow([a])
+    assert moved == [(c.pages_of(b), c.pages_of(a))]
+    c.free(a)
+    moved.clear()
+    c.grow([b])
+    assert not moved
+    consistent(c)
+
+
+def test_out_of_pages_changes_nothing(moved):
+    c = cache(pages=3)
+    a = c.add()
+    c.grow([a], 10)
+    b = c.fork(a)
+    before = (c.pages_of(a), c.length(a), c.free_pages)
+    for n in (1, 3):  # b would need a copy; a copy and a page
+        with pytest.raises(MemoryError):
+            c.grow([b], n)
+    with pytest.raises(MemoryError):
+        c.grow([a, b])
+    assert before == (c.pages_of(a), c.length(a), c.free_pages) and not moved
+    consistent(c)
+
+
+def test_refusals(moved):
+    c = cache()
+    a = c.add()
+    for bad in (lambda: c.grow([a, a]), lambda: c.grow([a], -1), lambda: c.grow([a], [1, 2]), lambda: cache(pages=0),
+                lambda: kvcache.PagedKVCache(1, 4, 1, 96, device="cpu"), lambda: cache(dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            bad()
+    assert c.length(a) == 0
+
+
+def test_compact(moved):
+    c = cache()
+    s = [c.add() for _ in range(4)]
+    for x in s:
+        c.grow([x], 8)
+    t = c.fork(s[3])
+    c.free(s[0])
+    c.free(s[2])
+    assert c.compact() == 4
+    (src, dst), = moved
+    assert not set(src) & set(dst) and max(dst) < 4 and min(src) >= 4
+    assert c.pages_of(t) == c.pages_of(s[3]) and max(c.pages_of(t) + c.pages_of(s[1])) < 4
+    consistent(c)
+    moved.clear()
+    assert c.compact() == 4 and not moved
+    c.grow([t])
+    consistent(c)
+
+
+def test_batch(moved):
+    c = cache()
+    a, b, e = c.add(), c.add(), c.add()
+    c.grow([a], 9)
+    c.grow([b, a], [2, 1])
+    got = c.batch([b, e, a])
+    assert got.table.tolist() == [c.pages_of(b) + [-1, -1], [-1] * 3, c.pages_of(a)]
+    assert got.lengths.tolist() == [2, 0, 10] and got.start.tolist() == [0, 0, 9] and got.count.tolist() == [2, 0, 1]
+    assert c.batch([]).table.shape == (0, 1)
