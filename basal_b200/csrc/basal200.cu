@@ -15,6 +15,7 @@
 #include "hybrid.cuh"
 #include "gdn_chunk.cuh"
 #include "paged.cuh"
+#include "attend.cuh"
 #include "gdn_step.cuh"
 #include "constrain.cuh"
 
@@ -46,10 +47,11 @@ int current_device(int* dev) {
 // Bits of DeviceInfo::smem_set, one per kernel instantiation that needs more than the default shared memory.
 enum SmemSlot {
   kSlotBlock = 0, kSlotFp4 = 8, kSlotSmall = 14, kSlotSplit = 26, kSlotSplitQ = 30, kSlotLogits = 38, kSlotGlu = 50,
-  kSlotRes = 58, kSlotGdn = 62, kSlotLogitsTc = 64, kSlotGdnV = 76, kSlotGdnVO = 78
+  kSlotRes = 58, kSlotGdn = 62, kSlotLogitsTc = 64, kSlotGdnV = 76, kSlotGdnVO = 78, kSlotAttend = 80
 };
 // kSlotFp4 .. + 5, kSlotSmall .. + 11, kSlotSplit .. + 3, kSlotSplitQ .. + 7, kSlotLogits .. + 11, kSlotGlu .. + 7,
-// kSlotRes .. + 3, kSlotGdn, kSlotLogitsTc .. + 11, kSlotGdnV .. + 1, kSlotGdnVO .. + 1 (bits of a 128-bit mask)
+// kSlotRes .. + 3, kSlotGdn, kSlotLogitsTc .. + 11, kSlotGdnV .. + 1, kSlotGdnVO .. + 1,
+// kSlotAttend .. + 19 (bits of a 128-bit mask)
 
 bool smem_is_set(int dev, int slot) { return (g_dev[dev].smem_set[slot >> 6] >> (slot & 63)) & 1; }
 
@@ -1137,12 +1139,52 @@ int check_cache(int dtype, int kv_dtype, int64_t page_stride, int64_t head_strid
   return BASAL200_OK;
 }
 
-template <typename TQ, typename TK>
-int attend_launch(const paged::AttendParams& p, int D, cudaStream_t st) {
-  const dim3 grid(p.H, p.rows);
-  if (D == 64) return launch_pdl(paged::attend_simple_kernel<TQ, TK, 64>, grid, 128, 0, st, p);
-  if (D == 128) return launch_pdl(paged::attend_simple_kernel<TQ, TK, 128>, grid, 128, 0, st, p);
-  return launch_pdl(paged::attend_simple_kernel<TQ, TK, 256>, grid, 128, 0, st, p);
+// Tiles of positions that a row can have, from its table's width and the window.
+int64_t attend_tiles(int64_t width, int64_t page_size, int64_t window) {
+  const int64_t nt = (width * page_size + paged::TILE - 1) / paged::TILE;
+  const int64_t in = window / paged::TILE + 2;
+  return window > 0 && in < nt ? in : nt;
+}
+
+int64_t attend_workspace(int64_t rows, int64_t H, int64_t D, int64_t width, int64_t page_size, int64_t window) {
+  const int parts = paged::most_parts((int)attend_tiles(width, page_size, window));
+  return parts > 1 ? rows * H * parts * (D + 2) * 4 : 0;
+}
+
+template <typename TQ, bool FP8, int D, int NG>
+int attend_launch(int dev, int slot, const paged::AttendParams& p, void* workspace, cudaStream_t st) {
+  using Sh = paged::AttendShape<FP8, D, NG>;
+  const int G = p.H / p.Hk, groups = (G + 8 * NG - 1) / (8 * NG);
+  const int parts = paged::most_parts((int)attend_tiles(p.width, p.page_size, p.window));
+  paged::Workspace ws = {};
+  ws.parts = parts;
+  if (parts > 1) {
+    const int64_t n = (int64_t)p.rows * p.H * parts;
+    ws.o = static_cast<float*>(workspace);
+    ws.m = ws.o + n * D;
+    ws.l = ws.m + n;
+  }
+  int rc = set_smem(dev, slot, paged::attend_kernel<TQ, FP8, D, NG>, Sh::SMEM);
+  if (rc) return rc;
+  const int64_t items = (int64_t)p.rows * p.Hk * groups * parts, most = (int64_t)g_dev[dev].sms * Sh::PER_SM;
+  rc = launch_pdl(paged::attend_kernel<TQ, FP8, D, NG>, (unsigned)(items < most ? items : most), paged::AWARPS * 32,
+                  Sh::SMEM, st, p, ws, groups);
+  if (rc || parts == 1) return rc;
+  return launch_pdl(paged::attend_join_kernel<TQ, D>, dim3(p.H, p.rows), 256, 0, st, p, ws);
+}
+
+// Query heads that share a key / value head are taken 8 at a time (one n tile of the MMA), or 16 where there are more
+// and the accumulators fit (D <= 128).
+template <typename TQ, bool FP8>
+int attend_pick(int dev, int slot, const paged::AttendParams& p, int D, void* workspace, cudaStream_t st) {
+  const bool two = p.H / p.Hk > 8;
+  if (D == 64)
+    return two ? attend_launch<TQ, FP8, 64, 2>(dev, slot, p, workspace, st)
+               : attend_launch<TQ, FP8, 64, 1>(dev, slot + 1, p, workspace, st);
+  if (D == 128)
+    return two ? attend_launch<TQ, FP8, 128, 2>(dev, slot + 2, p, workspace, st)
+               : attend_launch<TQ, FP8, 128, 1>(dev, slot + 3, p, workspace, st);
+  return attend_launch<TQ, FP8, 256, 1>(dev, slot + 4, p, workspace, st);
 }
 
 int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int D, void* workspace,
@@ -1157,14 +1199,19 @@ int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int
   if ((p.width > 0 && !p.table) || (p.pages > 0 && (!p.k || !p.v))) return BASAL200_ERR_ARG;
   if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out) || p.q_row % 8 || p.q_head % 8)
     return BASAL200_ERR_ALIGN;
-  if (p.rows > 65535) return BASAL200_ERR_LIMIT;
+  if (p.rows > 65535 || p.H > 4096) return BASAL200_ERR_LIMIT;
+  const int64_t need = attend_workspace(p.rows, p.H, D, p.width, p.page_size, p.window);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return BASAL200_ERR_ARG;
+  if (need > 0 && !aligned16(workspace)) return BASAL200_ERR_ALIGN;
   int dev;
   rc = current_device(&dev);
   if (rc) return rc;
-  using bf16 = __nv_bfloat16;
+  const bool fp8 = kv_dtype == BASAL200_E4M3;
   if (q_dtype == BASAL200_BF16)
-    return kv_dtype == BASAL200_E4M3 ? attend_launch<bf16, uint8_t>(p, D, st) : attend_launch<bf16, bf16>(p, D, st);
-  return kv_dtype == BASAL200_E4M3 ? attend_launch<__half, uint8_t>(p, D, st) : attend_launch<__half, __half>(p, D, st);
+    return fp8 ? attend_pick<__nv_bfloat16, true>(dev, kSlotAttend, p, D, workspace, st)
+               : attend_pick<__nv_bfloat16, false>(dev, kSlotAttend + 5, p, D, workspace, st);
+  return fp8 ? attend_pick<__half, true>(dev, kSlotAttend + 10, p, D, workspace, st)
+             : attend_pick<__half, false>(dev, kSlotAttend + 15, p, D, workspace, st);
 }
 
 template <typename T, bool FP8>
@@ -1546,7 +1593,10 @@ int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t 
 
 int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int width, int page_size,
                                                  int window) {
-  return 0;
+  if (rows <= 0 || H <= 0 || Hk <= 0 || D <= 0 || width <= 0 || page_size <= 0 || window < 0 ||
+      (int64_t)width * page_size > INT32_MAX - 64)
+    return 0;
+  return b200::attend_workspace(rows, H, D, width, page_size, window);
 }
 
 int basal200_kv_append(const void* k, const void* v, int dtype, int64_t k_row, int64_t k_tok, int64_t k_head,

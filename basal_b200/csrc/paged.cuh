@@ -55,84 +55,6 @@ struct AttendParams {
   void* out;               // [rows, H, D]
 };
 
-// One new token's attention: o = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t - max), over the row's positions
-// first <= t < length. A CTA of 4 warps per (row, head); a warp takes every fourth position, a lane D / 32 dimensions,
-// and keeps its running maximum, sum and weighted values in fp32; the warps' parts are joined in warp order.
-template <typename TQ, typename TK, int D>
-__global__ void __launch_bounds__(128) attend_simple_kernel(const AttendParams p) {
-  pdl_wait();
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.x, b = blockIdx.y, kvh = h / (p.H / p.Hk);
-  const int64_t most = (int64_t)p.width * p.page_size;
-  int n = max(p.lengths[b], 0);
-  bool bad = n > most;
-  if (bad) n = (int)most;
-  const int first = p.window > 0 ? max(0, n - p.window) : 0;
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = widen(static_cast<const TQ*>(p.q)[b * p.q_row + h * p.q_head + lane * E + e]);
-    o[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int t = first + warp; t < n; t += 4) {
-    const int page = p.table[b * p.table_row + t / p.page_size];
-    if (page < 0 || page >= p.pages) {
-      bad = true;
-      continue;
-    }
-    const int off = t % p.page_size;
-    const int64_t at = page * p.page_stride + kvh * p.head_stride + off * p.token_stride + lane * E;
-    const int64_t sat = page * p.s_page + kvh * p.s_head + off;
-    float z = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) z = fmaf(q[e], widen(static_cast<const TK*>(p.k)[at + e]), z);
-#pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
-    z *= p.scale;
-    float sv = 1.0f;
-    if (sizeof(TK) == 1) {
-      z *= p.ks[sat];
-      sv = p.vs[sat];
-    }
-    const float mn = max_nan(m, z), ref = mn == -INFINITY ? 0.0f : mn;
-    const float a = expf(m - ref), w = expf(z - ref);
-    l = l * a + w;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * sv * widen(static_cast<const TK*>(p.v)[at + e]);
-  }
-  __shared__ float sm[4], sl[4], so[4][D];
-  __shared__ int sbad;
-  if (threadIdx.x == 0) sbad = 0;
-  __syncthreads();
-  if (bad) sbad = 1;
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-  __syncthreads();
-  if (sbad && threadIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadPage);
-  float top = -INFINITY;
-  for (int w = 0; w < 4; ++w) top = max_nan(top, sm[w]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float total = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-      const float f = expf(sm[w] - ref);
-      total += f * sl[w];
-      acc += f * so[w][d];
-    }
-    float y = total == 0.0f ? 0.0f : acc / total;
-    if (sbad) y = NAN;
-    static_cast<TQ*>(p.out)[((int64_t)b * p.H + h) * D + d] = narrow<TQ>(y);
-  }
-  pdl_launch();
-}
-
 // ---------------------------------------------------------------------------------------------------------------
 // New tokens into the pages: a warp per (row, token, head) of the keys and of the values, a lane D / 32 consecutive
 // values. 16-bit pools take the values' bits; 8-bit pools their codes and the token's scale, by the activation
