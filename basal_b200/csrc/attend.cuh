@@ -53,6 +53,15 @@ struct Workspace {
   int parts; // the second-last dimension
 };
 
+// x / d for 0 <= x < 2^31 by a multiplication (Granlund and Montgomery 1994): shift = ceil(log2 d), mul =
+// floor(2^32 (2^shift - d) / d) + 1, x / d = (mulhi(x, mul) + x) >> shift. Exact, and the sum stays below 2^32.
+struct Divide {
+  uint32_t mul, shift;
+};
+__device__ __forceinline__ int divide(int x, Divide d) {
+  return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift);
+}
+
 // A row's span of positions, from its length: n (clamped to the table), first, and whether it was too long.
 __device__ __forceinline__ bool row_span(const AttendParams& p, int b, int* n, int* first) {
   const int len = p.lengths[b];
@@ -67,6 +76,9 @@ __device__ __forceinline__ int tiles_of(int n, int first) { return (n + TILE - 1
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
@@ -175,7 +187,7 @@ enum { kHas = 1, kFirst = 2, kLast = 4, kTile = 8, kBad = 16 };
 
 template <typename TQ, bool FP8, int D, int NG>
 __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
-    attend_kernel(const AttendParams p, const Workspace ws, int groups) {
+    attend_kernel(const AttendParams p, const Workspace ws, int groups, const Divide by_page) {
   using Sh = AttendShape<FP8, D, NG>;
   using TM = typename std::conditional<FP8, __half, TQ>::type;
   using MM = Mma<TM>;
@@ -211,9 +223,14 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
   bool it_bad = false, active = false, fresh = false;
   int page_at = 0, page_id = -1, page_lim = 0;  // page_id: table entry page_at + lane
 
-  const char* kbase = static_cast<const char*>(p.k);
-  const char* vbase = static_cast<const char*>(p.v);
   constexpr int ES = FP8 ? 1 : 2;
+  // a lane loads 16-byte chunk ch of token rows rr, rr + ROWS_STEP, ..
+  const int ch = lane % CH, rr = lane / CH;
+  const int64_t tok_bytes = p.token_stride * ES, step_bytes = tok_bytes * ROWS_STEP;
+  const char* const kbase = static_cast<const char*>(p.k) + ch * 16;
+  const char* const vbase = static_cast<const char*>(p.v) + ch * 16;
+  const bool whole_pages = p.page_size % TILE == 0;  // a tile lies in one page
+  int64_t head_bytes = 0, head_scales = 0;
 
   auto next_item = [&]() -> bool {
     while (item >= base + total) {
@@ -256,7 +273,9 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
     tile = t0 + it_part * per + warp;
     tile_end = t0 + min(nt, (it_part + 1) * per);
     page_at = -64;
-    page_lim = (it_n + p.page_size - 1) / p.page_size;
+    page_lim = divide(it_n + p.page_size - 1, by_page);
+    head_bytes = (it_unit / groups) * p.head_stride * ES;
+    head_scales = (it_unit / groups) * p.s_head;
     item += gridDim.x;
     return true;
   };
@@ -281,43 +300,54 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
                 (it_bad ? kBad : 0);
       if (has) {
         const int pos0 = tile * TILE;
-        // the pages of the tile's positions: 32 table entries at a time, one a lane
-        const int mine = pos0 + (lane & 15);
-        const bool live = mine >= it_first && mine < it_n;
         const int lo_pos = max(pos0, it_first), hi_pos = min(pos0 + TILE, it_n) - 1;
-        const int need_lo = lo_pos / p.page_size, need_hi = hi_pos / p.page_size;
+        const int need_lo = divide(lo_pos, by_page), need_hi = whole_pages ? need_lo : divide(hi_pos, by_page);
+        // the pages of the tile's positions: 32 table entries at a time, one a lane
         if (need_lo < page_at || need_hi >= page_at + 32) {
           page_at = need_lo;
           page_id = page_at + lane < page_lim ? p.table[it_row * p.table_row + page_at + lane] : -1;
         }
-        int pi, off;
-        if (need_lo == need_hi) {
-          pi = need_lo;
-          off = mine - need_lo * p.page_size;
-        } else {
-          pi = mine / p.page_size;
-          off = mine - pi * p.page_size;
-        }
-        const int page = __shfl_sync(0xffffffffu, page_id, (pi - page_at) & 31);
-        const bool fine = live && page >= 0 && page < p.pages;
-        if (__any_sync(0xffffffffu, live && !fine)) m.flags |= kBad;
-        const int kvh = it_unit / groups;
-        const int64_t at = fine ? (page * p.page_stride + kvh * p.head_stride + off * p.token_stride) * ES : -1;
         const uint32_t dst = smem_u32(ring + slot * Sh::STAGE);
-        const int ch = lane % CH, rr = lane / CH;
+        const int one = __shfl_sync(0xffffffffu, page_id, need_lo - page_at);
+        if (whole_pages && lo_pos == pos0 && hi_pos == pos0 + TILE - 1 && one >= 0 && one < p.pages) {
+          // a whole tile in one page: the same copies with the rows a stride apart
+          const int off = pos0 - need_lo * p.page_size;
+          int64_t at = one * p.page_stride * ES + head_bytes + (off + rr) * tok_bytes;
+          const uint32_t to = dst + rr * RB;
 #pragma unroll
-        for (int i = 0; i < TILE / ROWS_STEP; ++i) {
-          const int row = i * ROWS_STEP + rr;
-          const int64_t a = __shfl_sync(0xffffffffu, at, row);
-          const bool ok = a >= 0;
-          const int64_t g = (ok ? a : 0) + ch * 16;
-          const int ks = CH >= 8 ? (row & 1) << 2 : 0, vs = CH >= 8 ? row & 6 : (row >> 1) & 3;
-          cp_async16(dst + row * RB + ((ch ^ ks) << 4), kbase + g, ok);
-          cp_async16(dst + TILE * RB + row * RB + ((ch ^ vs) << 4), vbase + g, ok);
-        }
-        if (FP8) {
-          const float* s = lane < 16 ? p.ks : p.vs;
-          cp_async4(dst + 2 * TILE * RB + lane * 4, s + (fine ? page * p.s_page + kvh * p.s_head + off : 0), fine);
+          for (int i = 0; i < TILE / ROWS_STEP; ++i) {
+            const int row = i * ROWS_STEP + rr;
+            const int ks = CH >= 8 ? (row & 1) << 2 : 0, vs = CH >= 8 ? row & 6 : (row >> 1) & 3;
+            cp_async16(to + i * ROWS_STEP * RB + ((ch ^ ks) << 4), kbase + at);
+            cp_async16(to + (TILE + i * ROWS_STEP) * RB + ((ch ^ vs) << 4), vbase + at);
+            at += step_bytes;
+          }
+          if (FP8) {
+            const int64_t s = one * p.s_page + head_scales + off + (lane & 15);
+            cp_async4(dst + 2 * TILE * RB + lane * 4, (lane < 16 ? p.ks : p.vs) + s, true);
+          }
+        } else {
+          // the row's ends, and tiles that cross pages: each token's page on its own, zeros where there is none
+          const int mine = pos0 + (lane & 15);
+          const bool live = mine >= it_first && mine < it_n;
+          const int pi = live ? divide(mine, by_page) : need_lo;
+          const int off = mine - pi * p.page_size;
+          const int page = __shfl_sync(0xffffffffu, page_id, pi - page_at);
+          const bool fine = live && page >= 0 && page < p.pages;
+          if (__any_sync(0xffffffffu, live && !fine)) m.flags |= kBad;
+          const int64_t at = fine ? page * p.page_stride * ES + head_bytes + off * tok_bytes : -1;
+#pragma unroll 1
+          for (int row = rr; row < TILE; row += ROWS_STEP) {
+            const int64_t a = __shfl_sync(0xffffffffu, at, row);
+            const int64_t g = a >= 0 ? a : 0;
+            const int ks = CH >= 8 ? (row & 1) << 2 : 0, vs = CH >= 8 ? row & 6 : (row >> 1) & 3;
+            cp_async16(dst + row * RB + ((ch ^ ks) << 4), kbase + g, a >= 0);
+            cp_async16(dst + (TILE + row) * RB + ((ch ^ vs) << 4), vbase + g, a >= 0);
+          }
+          if (FP8) {
+            const int64_t s = fine ? page * p.s_page + head_scales + off : 0;
+            cp_async4(dst + 2 * TILE * RB + lane * 4, (lane < 16 ? p.ks : p.vs) + s, fine);
+          }
         }
       }
       fresh = false;
