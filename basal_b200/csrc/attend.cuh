@@ -13,14 +13,16 @@
 // written at once; parts of longer rows go to the workspace and attend_join_kernel adds them up.
 //
 // Arithmetic, per tile: S^T [16 tokens x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T on mma.sync m16n8k16 with
-// fp32 accumulators (8 heads fill the n side; tcgen05 would want 64 rows or more of a tile that has G). A product of
-// the dot product's D terms may be taken in any order, so a lane feeds the 16 bytes it loads straight to the MMA: the
-// k index of a step stands for the dimensions that the lane holds, the same for K and Q. V's pairs of tokens are
-// put together by byte permutes; P^T is moved into place by movmatrix. The weights are split into two 16-bit
-// values (p = hi + lo, 2^-17 of p lost), so the rounding of p does not show beside the output's own; running maximum,
-// sum and output stay in fp32, base 2. 8-bit pages: codes become fp16 exactly; a key's scale multiplies its logit, a
-// value's scale its weight, relative to a power of two that follows the largest scale seen, and the query is brought
-// to fp16 by a power of two of its own, so neither can leave fp16's range.
+// fp32 accumulators (8 heads fill the n side; tcgen05 would want 64 rows or more of a tile that has G). 16-bit pages
+// reach the MMA by ldmatrix (V transposed). 8-bit pages: codes become fp16 exactly; the products of a dot product may
+// be taken in any order, so the k index of a step stands for the dimensions whose bytes a lane holds, the same for K
+// and Q, and V's pairs of tokens are put together by byte permutes. P^T is moved into place by movmatrix, and split into
+// two 16-bit values (p = hi + lo, 2^-17 of p lost), so the rounding of p does not show beside the output's own.
+// Weights are 2^(z - ref) with z the logit times log2 e and ref a maximum that is raised only when some z passes it by
+// more than 8: a tile then costs one vote instead of a maximum across lanes and a rescaling of the sums, and weights
+// stay below 2^8, which changes no relative error (sums and outputs are fp32). An 8-bit key's scale multiplies its
+// logit, a value's scale its weight, relative to a power of two that follows the largest scale seen; the query is
+// brought to fp16 by a power of two of its own; so neither can leave fp16's range.
 #pragma once
 #include "paged.cuh"
 
@@ -149,6 +151,17 @@ struct Mma<__half> {
   }
 };
 
+// Four 8 x 8 matrices of 16-bit values (lane l gives the address of row l % 8 of matrix l / 8); T: each transposed.
+template <bool T>
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&v)[4]) {
+  if (T)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+}
+
 // Two e4m3 codes (the low 16 bits) as two fp16 values, exactly.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xFFFFu), __NV_E4M3);
@@ -169,6 +182,13 @@ struct AttendShape {
   static constexpr int STAGE = 2 * TILE * RB + (FP8 ? 2 * TILE * 4 : 0);
   // stages a warp: about 24 KB for each of 8 warps on an SM (two CTAs), 48 KB for each of 4 where D is 256
   static constexpr int STAGES = (D == 256 ? 49152 : 24576 + 512) / STAGE < 8 ? (D == 256 ? 49152 : 24576 + 512) / STAGE : 8;
+  // where a 16-byte chunk of token row `row` of a tile goes, so that the reads of a warp hit different banks
+  static __host__ __device__ constexpr int k_chunk(int ch, int row) {
+    return FP8 ? (CH >= 8 ? ch ^ ((row & 1) << 2) : ch) : ch ^ (row & 7);
+  }
+  static __host__ __device__ constexpr int v_chunk(int ch, int row) {
+    return FP8 ? (CH >= 8 ? ch ^ (row & 6) : ch ^ ((row >> 1) & 3)) : ch ^ (row & 7);
+  }
   static constexpr int JOIN = AWARPS * 8 * (D + 2) * 4 + 16;  // the warps' parts of 8 heads
   static constexpr int RING = AWARPS * STAGES * STAGE;
   static constexpr int META = AWARPS * STAGES * 32;
@@ -183,26 +203,28 @@ struct StageMeta {
   int at, n, first;      // the tile's first position, and the row's span
   int parts;             // items of the row
 };
+// The reference before any logit: finite, so that a difference with it is never NaN.
+constexpr float NO_MAX = -3.0e38f;
+constexpr float SLACK = 8.0f;
 enum { kHas = 1, kFirst = 2, kLast = 4, kTile = 8, kBad = 16 };
 
 template <typename TQ, bool FP8, int D, int NG>
 __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
-    attend_kernel(const AttendParams p, const Workspace ws, int groups, const Divide by_page) {
+    attend_kernel(const AttendParams p, const Workspace ws, int groups, const Divide by_page,
+                  const Divide by_unit) {
   using Sh = AttendShape<FP8, D, NG>;
   using TM = typename std::conditional<FP8, __half, TQ>::type;
   using MM = Mma<TM>;
   constexpr int STAGES = Sh::STAGES, CH = Sh::CH, RB = Sh::RB;
   constexpr int ROWS_STEP = 32 / CH;                 // token rows that one warp-wide load covers
-  constexpr int JC = CH / 4;                         // 16-byte chunks of a key that a lane feeds to the MMA
-  constexpr int QR = FP8 ? 8 : 4;                    // query registers that go with a chunk
-  constexpr int VB = RB / 8 < 16 ? RB / 8 : 16;      // bytes of a value load
+  constexpr int JC = CH / 4;                         // 8-bit: 16-byte chunks of a key that a lane feeds to the MMA
+  constexpr int VB = RB / 8 < 16 ? RB / 8 : 16;      // 8-bit: bytes of a value load
   constexpr int NV = RB / 8 / VB;                    // of them a token
-  constexpr int VE = VB / (FP8 ? 1 : 2);             // elements of one
   constexpr int MT = D / 16;                         // m tiles of O^T
 
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = lane >> 2, c = lane & 3;
+  const int r = lane >> 2, c = lane & 3, r8 = lane & 7, mat = lane >> 3;
   uint8_t* ring = smem + warp * STAGES * Sh::STAGE;
   StageMeta* meta = reinterpret_cast<StageMeta*>(smem + Sh::RING) + warp * STAGES;
   float* join_o = reinterpret_cast<float*>(smem + Sh::RING + Sh::META);  // [warp][8][D]
@@ -217,7 +239,7 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
 
   // ---- the loading side: items in order, their tiles, one stage a call ----
   int64_t item = blockIdx.x, base = 0;
-  int blk = -32, total = 0, incl = 0, row_n = 0, row_first = 0;
+  int blk = -32, total = 0, incl = 0, row_n = 0, row_first = 0, row_parts = 0;
   bool row_bad = false;
   int it_row = 0, it_unit = 0, it_part = 0, it_parts = 0, it_n = 0, it_first = 0, tile = 0, tile_end = 0;
   bool it_bad = false, active = false, fresh = false;
@@ -242,14 +264,13 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
         return false;
       }
       const int b = blk + lane;
-      int u = 0;
-      row_n = row_first = 0;
+      row_n = row_first = row_parts = 0;
       row_bad = false;
       if (b < p.rows) {
         row_bad = row_span(p, b, &row_n, &row_first);
-        u = parts_of(tiles_of(row_n, row_first)) * units;
+        row_parts = parts_of(tiles_of(row_n, row_first));
       }
-      incl = u;
+      incl = row_parts * units;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -265,10 +286,10 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
     const int before = who ? __shfl_sync(0xffffffffu, incl, who - 1) : 0;
     const int k = local - before;
     it_row = blk + who;
-    it_unit = k % units;
-    it_part = k / units;
+    it_part = divide(k, by_unit);
+    it_unit = k - it_part * units;
     const int nt = tiles_of(it_n, it_first);
-    it_parts = parts_of(nt);
+    it_parts = __shfl_sync(0xffffffffu, row_parts, who);
     const int per = tiles_per_item(nt), t0 = it_first / TILE;
     tile = t0 + it_part * per + warp;
     tile_end = t0 + min(nt, (it_part + 1) * per);
@@ -312,16 +333,21 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
         if (whole_pages && lo_pos == pos0 && hi_pos == pos0 + TILE - 1 && one >= 0 && one < p.pages) {
           // a whole tile in one page: the same copies with the rows a stride apart
           const int off = pos0 - need_lo * p.page_size;
-          int64_t at = one * p.page_stride * ES + head_bytes + (off + rr) * tok_bytes;
+          const int64_t at = one * p.page_stride * ES + head_bytes + (off + rr) * tok_bytes;
+          const char *kp = kbase + at, *vp = vbase + at;
           const uint32_t to = dst + rr * RB;
+          auto copy = [&](auto step) {
 #pragma unroll
-          for (int i = 0; i < TILE / ROWS_STEP; ++i) {
-            const int row = i * ROWS_STEP + rr;
-            const int ks = CH >= 8 ? (row & 1) << 2 : 0, vs = CH >= 8 ? row & 6 : (row >> 1) & 3;
-            cp_async16(to + i * ROWS_STEP * RB + ((ch ^ ks) << 4), kbase + at);
-            cp_async16(to + (TILE + i * ROWS_STEP) * RB + ((ch ^ vs) << 4), vbase + at);
-            at += step_bytes;
-          }
+            for (int i = 0; i < TILE / ROWS_STEP; ++i) {
+              const int row = i * ROWS_STEP + rr;
+              cp_async16(to + i * ROWS_STEP * RB + (Sh::k_chunk(ch, row) << 4), kp + i * step);
+              cp_async16(to + (TILE + i * ROWS_STEP) * RB + (Sh::v_chunk(ch, row) << 4), vp + i * step);
+            }
+          };
+          if (tok_bytes == RB)  // a head's tokens one after another: offsets known at compile time
+            copy(std::integral_constant<int, ROWS_STEP * RB>{});
+          else
+            copy(step_bytes);
           if (FP8) {
             const int64_t s = one * p.s_page + head_scales + off + (lane & 15);
             cp_async4(dst + 2 * TILE * RB + lane * 4, (lane < 16 ? p.ks : p.vs) + s, true);
@@ -340,9 +366,8 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
           for (int row = rr; row < TILE; row += ROWS_STEP) {
             const int64_t a = __shfl_sync(0xffffffffu, at, row);
             const int64_t g = a >= 0 ? a : 0;
-            const int ks = CH >= 8 ? (row & 1) << 2 : 0, vs = CH >= 8 ? row & 6 : (row >> 1) & 3;
-            cp_async16(dst + row * RB + ((ch ^ ks) << 4), kbase + g, a >= 0);
-            cp_async16(dst + (TILE + row) * RB + ((ch ^ vs) << 4), vbase + g, a >= 0);
+            cp_async16(dst + row * RB + (Sh::k_chunk(ch, row) << 4), kbase + g, a >= 0);
+            cp_async16(dst + (TILE + row) * RB + (Sh::v_chunk(ch, row) << 4), vbase + g, a >= 0);
           }
           if (FP8) {
             const int64_t s = fine ? page * p.s_page + head_scales + off : 0;
@@ -359,8 +384,8 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
   };
 
   // ---- the computing side ----
-  uint32_t q[NG][JC * QR];
-  float o[NG][MT][4], mx[NG][2], sum[NG][2], fac[NG][2];
+  uint32_t q[NG][D / 8];
+  float o[NG][MT][4], mx[NG][2], sum[NG][2], fac[NG][2];  // mx: the weights' reference, base 2
   float ref_v = 0.0f;  // 8-bit: the power of two that the values' scales are relative to
   bool refused = false;
 
@@ -388,13 +413,9 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
         float f = p.scale * 1.4426950408889634f;
         if constexpr (!FP8) {
 #pragma unroll
-          for (int j = 0; j < JC; ++j) {
-            uint4 u = *reinterpret_cast<const uint4*>(src + (j * 4 + c) * 8);
-            if (!live) u = make_uint4(0, 0, 0, 0);
-            q[g][j * 4] = u.x;
-            q[g][j * 4 + 1] = u.y;
-            q[g][j * 4 + 2] = u.z;
-            q[g][j * 4 + 3] = u.w;
+          for (int j = 0; j < D / 8; ++j) {  // step j / 2: dimensions 8 j + 2c, 8 j + 2c + 1
+            const uint32_t u = *reinterpret_cast<const uint32_t*>(src + j * 8 + 2 * c);
+            q[g][j] = live ? u : 0u;
           }
         } else {
           // the head's query over a power of two near its largest value, in fp16 (what falls below fp16's smallest
@@ -428,7 +449,7 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
         }
         fac[g][0] = __shfl_sync(0xffffffffu, f, c * 8);      // head 2c: lanes of row 2c
         fac[g][1] = __shfl_sync(0xffffffffu, f, c * 8 + 4);  // head 2c + 1
-        mx[g][0] = mx[g][1] = -INFINITY;
+        mx[g][0] = mx[g][1] = NO_MAX;
         sum[g][0] = sum[g][1] = 0.0f;
 #pragma unroll
         for (int t = 0; t < MT; ++t) o[g][t][0] = o[g][t][1] = o[g][t][2] = o[g][t][3] = 0.0f;
@@ -438,142 +459,159 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
 
     if (flags & kTile) {
       const uint32_t ks = smem_u32(ring + slot * Sh::STAGE), vs = ks + TILE * RB;
-      float s[NG][4];
+      float s[NG][4], s2[NG][4];  // two sums, taken in turn: shorter chains of dependent MMAs
 #pragma unroll
-      for (int g = 0; g < NG; ++g) s[g][0] = s[g][1] = s[g][2] = s[g][3] = 0.0f;
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int j = 0; j < JC; ++j) {
-        const uint32_t ch = (uint32_t)(j * 4 + c) ^ (CH >= 8 ? (r & 1) << 2 : 0);
-        const uint4 a = lds16(ks + r * RB + (ch << 4)), b = lds16(ks + (r + 8) * RB + (ch << 4));
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-        if constexpr (!FP8) {
+        for (int i = 0; i < 4; ++i) s[g][i] = s2[g][i] = 0.0f;
+      if constexpr (!FP8) {
+        const uint32_t a = (ks + (r8 + (mat & 1) * 8) * RB) + (((mat >> 1) ^ r8) << 4);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            MM::run(s[g], aw[0], bw[0], aw[1], bw[1], q[g][j * 4], q[g][j * 4 + 1]);
-            MM::run(s[g], aw[2], bw[2], aw[3], bw[3], q[g][j * 4 + 2], q[g][j * 4 + 3]);
-          }
-        } else {
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t k[4];
+          ldmatrix4<false>(a ^ (j << 5), k);
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            MM::run(j & 1 ? s2[g] : s[g], k[0], k[1], k[2], k[3], q[g][2 * j], q[g][2 * j + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < JC; ++j) {
+          const int chunk = j * 4 + c;
+          const uint4 a = lds16(ks + r * RB + (Sh::k_chunk(chunk, r) << 4)),
+                      b = lds16(ks + (r + 8) * RB + (Sh::k_chunk(chunk, r) << 4));
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t a0 = codes_f16(aw[w]), a1 = codes_f16(bw[w]), a2 = codes_f16(aw[w] >> 16),
                            a3 = codes_f16(bw[w] >> 16);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) MM::run(s[g], a0, a1, a2, a3, q[g][j * 8 + 2 * w], q[g][j * 8 + 2 * w + 1]);
+            for (int g = 0; g < NG; ++g)
+              MM::run(w & 1 ? s2[g] : s[g], a0, a1, a2, a3, q[g][j * 8 + 2 * w], q[g][j * 8 + 2 * w + 1]);
           }
         }
       }
       // the logits, base 2: rows are tokens at + r and at + r + 8, columns heads 2c and 2c + 1
-      float k0 = 1.0f, k1 = 1.0f, v0 = 1.0f, v1 = 1.0f, grow = 1.0f;
+      float k0 = 1.0f, k1 = 1.0f, v0 = 1.0f, v1 = 1.0f, top_v = 0.0f;
       if (FP8) {
         const uint32_t sc = ks + 2 * TILE * RB;
         k0 = lds_f(sc + r * 4);
         k1 = lds_f(sc + r * 4 + 32);
         v0 = lds_f(sc + 64 + r * 4);
         v1 = lds_f(sc + 64 + r * 4 + 32);
-        float top = fmaxf(fabsf(v0), fabsf(v1));
+        top_v = fmaxf(fabsf(v0), fabsf(v1));
+      }
+      const bool edge = at < first || at + TILE > n;
+      float z[NG][4];
+      bool up = FP8 && top_v > ref_v;
 #pragma unroll
-        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        if (top > ref_v) {  // uniform over the warp
-          const uint32_t e = min((__float_as_uint(top) >> 23) + 2u, 253u);
-          const float now = __uint_as_float(e << 23), inv = __uint_as_float((254u - e) << 23);
-          grow = ref_v * inv;
-          ref_v = now;
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          z[g][i] = (s[g][i] + s2[g][i]) * fac[g][i & 1];
+          if (FP8) z[g][i] *= i < 2 ? k0 : k1;
         }
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pos = at + r + (i < 2 ? 0 : 8);
+            z[g][i] = pos >= first && pos < n ? z[g][i] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) up |= fmaxf(z[g][h], z[g][h + 2]) > mx[g][h] + SLACK;
+      }
+      if (__any_sync(0xffffffffu, up)) {  // raise the references to what has been seen, and the sums with them
+        float grow = 1.0f;
+        if (FP8) {
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, x));
+          if (top_v > ref_v) {
+            const uint32_t e = min((__float_as_uint(top_v) >> 23) + 2u, 253u);
+            grow = ref_v * __uint_as_float((254u - e) << 23);
+            ref_v = __uint_as_float(e << 23);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float m = fmaxf(z[g][h], z[g][h + 2]);
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            m = fmaxf(m, mx[g][h]);
+            float f = ex2(mx[g][h] - m);
+            mx[g][h] = m;
+            sum[g][h] *= f;
+            f *= grow;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[g][i][h] *= f;
+              o[g][i][h + 2] *= f;
+            }
+          }
+      }
+      if (FP8) {
         const float inv = ref_v > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref_v)) : 0.0f;
         v0 *= inv;
         v1 *= inv;
       }
-      const bool edge = at < first || at + TILE > n;
-      const bool in0 = at + r >= first && at + r < n, in1 = at + r + 8 >= first && at + r + 8 < n;
       uint32_t ph[NG][2], pl[NG][2];
-      float al[NG][2];
-      bool moved = FP8 && grow != 1.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float z[4] = {s[g][0] * fac[g][0], s[g][1] * fac[g][1], s[g][2] * fac[g][0], s[g][3] * fac[g][1]};
-        if (FP8) {
-          z[0] *= k0;
-          z[1] *= k0;
-          z[2] *= k1;
-          z[3] *= k1;
-        }
-        if (edge) {
-          z[0] = in0 ? z[0] : -INFINITY;
-          z[1] = in0 ? z[1] : -INFINITY;
-          z[2] = in1 ? z[2] : -INFINITY;
-          z[3] = in1 ? z[3] : -INFINITY;
-        }
+        float w[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float t = fmaxf(z[h], z[h + 2]);
-#pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-          t = fmaxf(t, mx[g][h]);
-          const float ref = t == -INFINITY ? 0.0f : t;
-          al[g][h] = ex2(mx[g][h] - ref);
-          moved |= t != mx[g][h];
-          mx[g][h] = t;
-          z[h] = ex2(z[h] - ref);
-          z[h + 2] = ex2(z[h + 2] - ref);
-          sum[g][h] = fmaf(sum[g][h], al[g][h], z[h] + z[h + 2]);
-          if (FP8) al[g][h] *= grow;
-        }
+        for (int i = 0; i < 4; ++i) w[i] = ex2(z[g][i] - mx[g][i & 1]);
+        sum[g][0] += w[0] + w[2];
+        sum[g][1] += w[1] + w[3];
         if (FP8) {
-          z[0] *= v0;
-          z[1] *= v0;
-          z[2] *= v1;
-          z[3] *= v1;
+          w[0] *= v0;
+          w[1] *= v0;
+          w[2] *= v1;
+          w[3] *= v1;
         }
-        const uint32_t h0 = MM::pack(z[0], z[1]), h1 = MM::pack(z[2], z[3]);
+        const uint32_t h0 = MM::pack(w[0], w[1]), h1 = MM::pack(w[2], w[3]);
         const float2 f0 = MM::unpack(h0), f1 = MM::unpack(h1);
         ph[g][0] = transposed(h0);
         ph[g][1] = transposed(h1);
-        pl[g][0] = transposed(MM::pack(z[0] - f0.x, z[1] - f0.y));
-        pl[g][1] = transposed(MM::pack(z[2] - f1.x, z[3] - f1.y));
+        pl[g][0] = transposed(MM::pack(w[0] - f0.x, w[1] - f0.y));
+        pl[g][1] = transposed(MM::pack(w[2] - f1.x, w[3] - f1.y));
       }
-      if (__any_sync(0xffffffffu, moved)) {
+      // O^T += V^T P^T
+      if constexpr (!FP8) {
+        const uint32_t a = (vs + (r8 + (mat >> 1) * 8) * RB) + (((mat & 1) ^ r8) << 4);
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int j = 0; j < MT; ++j) {
+          uint32_t v[4];
+          ldmatrix4<true>(a ^ (j << 5), v);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            o[g][t][0] *= al[g][0];
-            o[g][t][1] *= al[g][1];
-            o[g][t][2] *= al[g][0];
-            o[g][t][3] *= al[g][1];
-          }
-      }
-      // O^T += V^T P^T: a lane takes piece i * 8 + r of tokens 2c, 2c + 1, 2c + 8, 2c + 9
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        uint32_t v[4][VB / 4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
-          if constexpr (VB == 16) {
-            const uint32_t ch = (uint32_t)(i * 8 + r) ^ (uint32_t)(tok & 6);
-            const uint4 u = lds16(vs + tok * RB + (ch << 4));
-            v[t][0] = u.x;
-            v[t][1] = u.y;
-            v[t][2] = u.z;
-            v[t][3] = u.w;
-          } else {
-            const uint32_t ch = (uint32_t)(r >> 1) ^ (uint32_t)((tok >> 1) & 3);
-            const uint2 u = lds8(vs + tok * RB + (ch << 4) + (r & 1) * 8);
-            v[t][0] = u.x;
-            v[t][1] = u.y;
+          for (int g = 0; g < NG; ++g) {
+            MM::run(o[g][j], v[0], v[1], v[2], v[3], ph[g][0], ph[g][1]);
+            MM::run(o[g][j], v[0], v[1], v[2], v[3], pl[g][0], pl[g][1]);
           }
         }
+      } else {
+        // a lane takes piece i * 8 + r of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
-        for (int w = 0; w < VB / 4; ++w) {
-          if constexpr (!FP8) {
-            const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
-            const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+        for (int i = 0; i < NV; ++i) {
+          uint32_t v[4][VB / 4];
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              MM::run(o[g][i * (VE / 2) + w], a0, a1, a2, a3, ph[g][0], ph[g][1]);
-              MM::run(o[g][i * (VE / 2) + w], a0, a1, a2, a3, pl[g][0], pl[g][1]);
+          for (int t = 0; t < 4; ++t) {
+            const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
+            if constexpr (VB == 16) {
+              const uint4 u = lds16(vs + tok * RB + (Sh::v_chunk(i * 8 + r, tok) << 4));
+              v[t][0] = u.x;
+              v[t][1] = u.y;
+              v[t][2] = u.z;
+              v[t][3] = u.w;
+            } else {
+              const uint2 u = lds8(vs + tok * RB + (Sh::v_chunk(r >> 1, tok) << 4) + (r & 1) * 8);
+              v[t][0] = u.x;
+              v[t][1] = u.y;
             }
-          } else {
+          }
+#pragma unroll
+          for (int w = 0; w < VB / 4; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t sel = h ? 0x7362 : 0x5140;
@@ -581,11 +619,10 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
               const uint32_t a0 = codes_f16(x), a1 = codes_f16(x >> 16), a2 = codes_f16(y), a3 = codes_f16(y >> 16);
 #pragma unroll
               for (int g = 0; g < NG; ++g) {
-                MM::run(o[g][i * (VE / 2) + w * 2 + h], a0, a1, a2, a3, ph[g][0], ph[g][1]);
-                MM::run(o[g][i * (VE / 2) + w * 2 + h], a0, a1, a2, a3, pl[g][0], pl[g][1]);
+                MM::run(o[g][i * (VB / 2) + w * 2 + h], a0, a1, a2, a3, ph[g][0], ph[g][1]);
+                MM::run(o[g][i * (VB / 2) + w * 2 + h], a0, a1, a2, a3, pl[g][0], pl[g][1]);
               }
             }
-          }
         }
       }
     }
@@ -608,9 +645,11 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
           if (head < live) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-              const int d = ((t / (VE / 2)) * 8 + r) * VE + (t % (VE / 2)) * 2;
-              *reinterpret_cast<float2*>(join_o + (warp * 8 + head) * D + d) =
-                  make_float2(o[g][t][h] * back, o[g][t][h + 2] * back);
+              // the rows r and r + 8 of m tile t
+              const int d0 = FP8 ? (t / (VB / 2) * 8 + r) * VB + t % (VB / 2) * 2 : t * 16 + r, d1 = d0 + (FP8 ? 1 : 8);
+              float* to = join_o + (warp * 8 + head) * D;
+              to[d0 ^ (c << 3)] = o[g][t][h] * back;  // c = head / 2: other banks for the other heads
+              to[d1 ^ (c << 3)] = o[g][t][h + 2] * back;
             }
           }
         }
@@ -620,12 +659,11 @@ __global__ void __launch_bounds__(AWARPS * 32, AttendShape<FP8, D, NG>::PER_SM)
           float top = join_m[head];
 #pragma unroll
           for (int w = 1; w < AWARPS; ++w) top = max_nan(top, join_m[w * 8 + head]);
-          const float ref = top == -INFINITY ? 0.0f : top;
           float l = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
           for (int w = 0; w < AWARPS; ++w) {
-            const float f = ex2(join_m[w * 8 + head] - ref);
-            const float2 v = *reinterpret_cast<const float2*>(join_o + (w * 8 + head) * D + d);
+            const float f = ex2(join_m[w * 8 + head] - top);
+            const float2 v = *reinterpret_cast<const float2*>(join_o + (w * 8 + head) * D + (d ^ (head >> 1 << 3)));
             l = fmaf(join_l[w * 8 + head], f, l);
             x = fmaf(v.x, f, x);
             y = fmaf(v.y, f, y);
@@ -669,7 +707,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p, 
   if (parts > 1) {
     const int64_t rh = (int64_t)b * p.H + h;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float m = (int)threadIdx.x < parts ? ws.m[rh * ws.parts + threadIdx.x] : -INFINITY;
+    const float m = (int)threadIdx.x < parts ? ws.m[rh * ws.parts + threadIdx.x] : NO_MAX;
     const float l = (int)threadIdx.x < parts ? ws.l[rh * ws.parts + threadIdx.x] : 0.0f;
     float top = m;
 #pragma unroll
@@ -678,8 +716,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendParams p, 
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) top = max_nan(top, red[w]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float f = ex2(m - ref);
+    const float f = ex2(m - top);
     weight[threadIdx.x] = f;
     float total = f * l;
 #pragma unroll

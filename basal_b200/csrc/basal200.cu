@@ -1151,6 +1151,12 @@ int64_t attend_workspace(int64_t rows, int64_t H, int64_t D, int64_t width, int6
   return parts > 1 ? rows * H * parts * (D + 2) * 4 : 0;
 }
 
+paged::Divide divider(int d) {
+  uint32_t shift = 0;
+  while ((1ll << shift) < d) ++shift;
+  return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
 template <typename TQ, bool FP8, int D, int NG>
 int attend_launch(int dev, int slot, const paged::AttendParams& p, void* workspace, cudaStream_t st) {
   using Sh = paged::AttendShape<FP8, D, NG>;
@@ -1167,11 +1173,8 @@ int attend_launch(int dev, int slot, const paged::AttendParams& p, void* workspa
   int rc = set_smem(dev, slot, paged::attend_kernel<TQ, FP8, D, NG>, Sh::SMEM);
   if (rc) return rc;
   const int64_t items = (int64_t)p.rows * p.Hk * groups * parts, most = (int64_t)g_dev[dev].sms * Sh::PER_SM;
-  uint32_t shift = 0;
-  while ((1ll << shift) < p.page_size) ++shift;
-  const paged::Divide by_page = {(uint32_t)((((1ull << shift) - p.page_size) << 32) / p.page_size + 1), shift};
   rc = launch_pdl(paged::attend_kernel<TQ, FP8, D, NG>, (unsigned)(items < most ? items : most), paged::AWARPS * 32,
-                  Sh::SMEM, st, p, ws, groups, by_page);
+                  Sh::SMEM, st, p, ws, groups, divider(p.page_size), divider(p.Hk * groups));
   if (rc || parts == 1) return rc;
   return launch_pdl(paged::attend_join_kernel<TQ, D>, dim3(p.H, p.rows), 256, 0, st, p, ws);
 }
