@@ -53,7 +53,7 @@ SIGNATURES = {
     "basal200_gdn_gate_fp8_quant": [_P, _I, _I, _P, _I, _I64, _I, _P, _F, _I, _I, _I, _P, _P, _P, _P],
     "basal200_paged_attention": [_P, _I, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _P,
                                  _I64, _I, _P, _I, _I, _I, _I, _F, _I, _P, _P, _I64, _P],
-    "basal200_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I],
+    "basal200_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
     "basal200_kv_append": [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _P, _I64,
                            _I64, _I64, _I, _P, _I64, _I, _P, _P, _I, _I, _I, _I, _P],
     "basal200_kv_copy_pages": [_P, _P, _P, _I, _I64, _P, _P, _I, _P],

@@ -1139,16 +1139,17 @@ int check_cache(int dtype, int kv_dtype, int64_t page_stride, int64_t head_strid
   return BASAL200_OK;
 }
 
-// Tiles of positions that a row can have, from its table's width and the window.
-int64_t attend_tiles(int64_t width, int64_t page_size, int64_t window) {
-  const int64_t nt = (width * page_size + paged::TILE - 1) / paged::TILE;
-  const int64_t in = window / paged::TILE + 2;
-  return window > 0 && in < nt ? in : nt;
-}
+// Query heads that share a key / value head are taken 8 at a time (one n tile of the MMA), or 16 where there are more
+// and the accumulators fit (D <= 128).
+int attend_ng(int H, int Hk, int D) { return H / Hk > 8 && D <= 128 ? 2 : 1; }
+int attend_groups(int H, int Hk, int D) { return (H / Hk + 8 * attend_ng(H, Hk, D) - 1) / (8 * attend_ng(H, Hk, D)); }
 
-int64_t attend_workspace(int64_t rows, int64_t H, int64_t D, int64_t width, int64_t page_size, int64_t window) {
-  const int parts = paged::most_parts((int)attend_tiles(width, page_size, window));
-  return parts > 1 ? rows * H * parts * (D + 2) * 4 : 0;
+// Parts that a row can have, from its table's width and the window.
+int attend_parts(int64_t width, int64_t page_size, int64_t window, bool fp8, int H, int Hk, int D) {
+  const int ng = attend_ng(H, Hk, D);
+  const int64_t tt = paged::tile_of(fp8, D, ng), nt = (width * page_size + tt - 1) / tt, in = window / tt + 2;
+  return paged::most_parts(window > 0 && in < nt ? in : nt, paged::item_tiles(fp8, D, ng),
+                           paged::parts_cap(D, ng, Hk * attend_groups(H, Hk, D)));
 }
 
 paged::Divide divider(int d) {
@@ -1160,10 +1161,11 @@ paged::Divide divider(int d) {
 template <typename TQ, bool FP8, int D, int NG>
 int attend_launch(int dev, int slot, const paged::AttendParams& p, void* workspace, cudaStream_t st) {
   using Sh = paged::AttendShape<FP8, D, NG>;
-  const int G = p.H / p.Hk, groups = (G + 8 * NG - 1) / (8 * NG);
-  const int parts = paged::most_parts((int)attend_tiles(p.width, p.page_size, p.window));
+  const int groups = attend_groups(p.H, p.Hk, D);
+  const int parts = attend_parts(p.width, p.page_size, p.window, FP8, p.H, p.Hk, D);
   paged::Workspace ws = {};
   ws.parts = parts;
+  ws.cap = paged::parts_cap(D, NG, p.Hk * groups);
   if (parts > 1) {
     const int64_t n = (int64_t)p.rows * p.H * parts;
     ws.o = static_cast<float*>(workspace);
@@ -1172,18 +1174,18 @@ int attend_launch(int dev, int slot, const paged::AttendParams& p, void* workspa
   }
   int rc = set_smem(dev, slot, paged::attend_kernel<TQ, FP8, D, NG>, Sh::SMEM);
   if (rc) return rc;
-  const int64_t items = (int64_t)p.rows * p.Hk * groups * parts, most = (int64_t)g_dev[dev].sms * Sh::PER_SM;
-  rc = launch_pdl(paged::attend_kernel<TQ, FP8, D, NG>, (unsigned)(items < most ? items : most), paged::AWARPS * 32,
-                  Sh::SMEM, st, p, ws, groups, divider(p.page_size), divider(p.Hk * groups));
+  const int64_t items = (int64_t)p.rows * p.Hk * groups * parts, most = (int64_t)g_dev[dev].sms * Sh::CTAS;
+  rc = launch_pdl(paged::attend_kernel<TQ, FP8, D, NG>, (unsigned)(items < most ? items : most), Sh::W * 32,
+                  Sh::SMEM, st, p, ws, groups, divider(p.page_size), divider(p.Hk * groups), divider(groups),
+                  divider(ws.cap));
   if (rc || parts == 1) return rc;
-  return launch_pdl(paged::attend_join_kernel<TQ, D>, dim3(p.H, p.rows), 256, 0, st, p, ws);
+  return launch_pdl(paged::attend_join_kernel<TQ, D, Sh::TT>, dim3(p.H, p.rows), 256, 0, st, p, ws,
+                    paged::item_tiles(FP8, D, NG));
 }
 
-// Query heads that share a key / value head are taken 8 at a time (one n tile of the MMA), or 16 where there are more
-// and the accumulators fit (D <= 128).
 template <typename TQ, bool FP8>
 int attend_pick(int dev, int slot, const paged::AttendParams& p, int D, void* workspace, cudaStream_t st) {
-  const bool two = p.H / p.Hk > 8;
+  const bool two = attend_ng(p.H, p.Hk, D) == 2;
   if (D == 64)
     return two ? attend_launch<TQ, FP8, 64, 2>(dev, slot, p, workspace, st)
                : attend_launch<TQ, FP8, 64, 1>(dev, slot + 1, p, workspace, st);
@@ -1206,13 +1208,14 @@ int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int
   if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out) || p.q_row % 8 || p.q_head % 8)
     return BASAL200_ERR_ALIGN;
   if (p.rows > 65535 || p.H > 4096) return BASAL200_ERR_LIMIT;
-  const int64_t need = attend_workspace(p.rows, p.H, D, p.width, p.page_size, p.window);
+  const bool fp8 = kv_dtype == BASAL200_E4M3;
+  const int parts = attend_parts(p.width, p.page_size, p.window, fp8, p.H, p.Hk, D);
+  const int64_t need = parts > 1 ? (int64_t)p.rows * p.H * parts * (D + 2) * 4 : 0;
   if (need > 0 && (!workspace || workspace_bytes < need)) return BASAL200_ERR_ARG;
   if (need > 0 && !aligned16(workspace)) return BASAL200_ERR_ALIGN;
   int dev;
   rc = current_device(&dev);
   if (rc) return rc;
-  const bool fp8 = kv_dtype == BASAL200_E4M3;
   if (q_dtype == BASAL200_BF16)
     return fp8 ? attend_pick<__nv_bfloat16, true>(dev, kSlotAttend, p, D, workspace, st)
                : attend_pick<__nv_bfloat16, false>(dev, kSlotAttend + 5, p, D, workspace, st);
@@ -1597,12 +1600,13 @@ int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t 
   return b200::paged_attention(p, q_dtype, kv_dtype, D, workspace, workspace_bytes, as_stream(stream));
 }
 
-int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int width, int page_size,
-                                                 int window) {
-  if (rows <= 0 || H <= 0 || Hk <= 0 || D <= 0 || width <= 0 || page_size <= 0 || window < 0 ||
+int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int kv_dtype, int width,
+                                                 int page_size, int window) {
+  if (rows <= 0 || H <= 0 || Hk <= 0 || H % Hk || (D != 64 && D != 128 && D != 256) || width <= 0 || page_size <= 0 || window < 0 ||
       (int64_t)width * page_size > INT32_MAX - 64)
     return 0;
-  return b200::attend_workspace(rows, H, D, width, page_size, window);
+  const int parts = b200::attend_parts(width, page_size, window, kv_dtype == BASAL200_E4M3, H, Hk, D);
+  return parts > 1 ? (int64_t)rows * H * parts * (D + 2) * 4 : 0;
 }
 
 int basal200_kv_append(const void* k, const void* v, int dtype, int64_t k_row, int64_t k_tok, int64_t k_head,

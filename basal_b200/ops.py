@@ -708,7 +708,7 @@ def _paged_attention(q, k_pages, v_pages, table, lengths, scale, window=0, k_sca
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
     out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
-    n = _lib.lib().basal200_paged_attention_workspace_bytes(rows, H, Hk, D, table.shape[1], ps, window)
+    n = _lib.lib().basal200_paged_attention_workspace_bytes(rows, H, Hk, D, kvt, table.shape[1], ps, window)
     work = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
     call("basal200_paged_attention", dev, ptr(q), code(q.dtype), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages),
          kvt, *cache, ptr(_c(lengths)), rows, H, Hk, D, scale, window, ptr(out), ptr(work), n)

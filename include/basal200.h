@@ -319,7 +319,8 @@ int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t 
 
 /* Workspace bytes of basal200_paged_attention for rows of up to width * page_size positions; 0: none is needed (NULL
  * allowed). Pure: no device call. */
-int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int width, int page_size, int window);
+int64_t basal200_paged_attention_workspace_bytes(int rows, int H, int Hk, int D, int kv_dtype, int width,
+                                                 int page_size, int window);
 
 /* Writes tokens t < min(T, count[b]) (count NULL: T) of row b's new keys and values (k, v [rows, T, Hk, D], dtype bf16
  * or fp16, element strides k_row, k_tok, k_head and v_...; D contiguous, 16-byte aligned) into the pools at positions
