@@ -47,11 +47,11 @@ int current_device(int* dev) {
 // Bits of DeviceInfo::smem_set, one per kernel instantiation that needs more than the default shared memory.
 enum SmemSlot {
   kSlotBlock = 0, kSlotFp4 = 8, kSlotSmall = 14, kSlotSplit = 26, kSlotSplitQ = 30, kSlotLogits = 38, kSlotGlu = 50,
-  kSlotRes = 58, kSlotGdn = 62, kSlotLogitsTc = 64, kSlotGdnV = 76, kSlotGdnVO = 78, kSlotAttend = 80
+  kSlotRes = 58, kSlotGdn = 62, kSlotLogitsTc = 64, kSlotGdnV = 76, kSlotGdnVO = 78, kSlotAttend = 80, kSlotConstrain = 100
 };
 // kSlotFp4 .. + 5, kSlotSmall .. + 11, kSlotSplit .. + 3, kSlotSplitQ .. + 7, kSlotLogits .. + 11, kSlotGlu .. + 7,
 // kSlotRes .. + 3, kSlotGdn, kSlotLogitsTc .. + 11, kSlotGdnV .. + 1, kSlotGdnVO .. + 1,
-// kSlotAttend .. + 19 (bits of a 128-bit mask)
+// kSlotAttend .. + 19, kSlotConstrain .. + 5 (bits of a 128-bit mask)
 
 bool smem_is_set(int dev, int slot) { return (g_dev[dev].smem_set[slot >> 6] >> (slot & 63)) & 1; }
 
@@ -146,6 +146,28 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return launched();
+  return launched();
+}
+
+// The same for a kernel whose CTAs form clusters of `cluster` along x.
+template <typename... KArgs, typename... Args>
+int launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, unsigned cluster,
+                       Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return launched();
   return launched();
 }
@@ -1225,11 +1247,10 @@ int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int
 
 template <typename T, bool FP8>
 int append_launch(const paged::AppendParams& p, int D, cudaStream_t st) {
-  const int64_t grid = ((int64_t)p.rows * p.T * p.Hk * 2 + 7) / 8;  // a warp each, 8 a CTA
-  if (grid > INT32_MAX) return BASAL200_ERR_LIMIT;
-  if (D == 64) return launch_pdl(paged::append_kernel<T, FP8, 64>, (unsigned)grid, 256, 0, st, p);
-  if (D == 128) return launch_pdl(paged::append_kernel<T, FP8, 128>, (unsigned)grid, 256, 0, st, p);
-  return launch_pdl(paged::append_kernel<T, FP8, 256>, (unsigned)grid, 256, 0, st, p);
+  const dim3 grid((p.T + paged::APPEND_TOKENS - 1) / paged::APPEND_TOKENS, p.rows);
+  if (D == 64) return launch_pdl(paged::append_kernel<T, FP8, 64>, grid, 256, 0, st, p);
+  if (D == 128) return launch_pdl(paged::append_kernel<T, FP8, 128>, grid, 256, 0, st, p);
+  return launch_pdl(paged::append_kernel<T, FP8, 256>, grid, 256, 0, st, p);
 }
 
 int kv_append(const paged::AppendParams& p, int dtype, int kv_dtype, int D, cudaStream_t st) {
@@ -1245,6 +1266,7 @@ int kv_append(const paged::AppendParams& p, int dtype, int kv_dtype, int D, cuda
     if (!aligned16(p.src[i]) || !aligned16(p.pool[i]) || p.row[i] % 8 || p.tok[i] % 8 || p.head[i] % 8)
       return BASAL200_ERR_ALIGN;
   }
+  if (p.rows > 65535 || p.Hk > 65535 || p.T > INT32_MAX - 64) return BASAL200_ERR_LIMIT;
   int dev;
   rc = current_device(&dev);
   if (rc) return rc;
@@ -1320,6 +1342,17 @@ int kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_byt
   return copy_pages_launch<1024>(pools, layers, page_bytes, npools, pages, src, dst, n, st);
 }
 
+#ifndef GDN_WIDE
+#define GDN_WIDE 2
+#endif
+// A cluster of 8 CTAs of 16 columns a (row, key head) while that many CTAs of 128 columns would leave SMs idle.
+template <typename T>
+int gdn_step_launch(const gdnstep::Params& p, int dev, cudaStream_t st) {
+  if ((int64_t)p.rows * p.Hk >= GDN_WIDE * g_dev[dev].sms)
+    return launch_pdl(gdnstep::gdn_step_kernel<T, 128, 256>, dim3(p.Hk, p.rows), 256, 0, st, p);
+  return launch_pdl_cluster(gdnstep::gdn_step_kernel<T, 16, 128>, dim3(p.Hk * 8, p.rows), 128, 0, st, 8, p);
+}
+
 int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   if (p.rows < 0 || p.Hk <= 0 || p.Hv <= 0 || p.slots < 0) return BASAL200_ERR_ARG;
   if (p.Hv % p.Hk) return BASAL200_ERR_SHAPE;
@@ -1337,9 +1370,25 @@ int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  if (dt == BASAL200_BF16)
-    return launch_pdl(gdnstep::gdn_step_kernel<__nv_bfloat16>, dim3(p.Hk, p.rows), 128, 0, st, p);
-  return launch_pdl(gdnstep::gdn_step_kernel<__half>, dim3(p.Hk, p.rows), 128, 0, st, p);
+  return dt == BASAL200_BF16 ? gdn_step_launch<__nv_bfloat16>(p, dev, st) : gdn_step_launch<__half>(p, dev, st);
+}
+
+// Slices of up to 16384 tokens (the history is read once a slice), smaller where few rows would leave SMs idle: about 4
+// CTAs an SM.
+template <typename T>
+int constrain_launch(constrain::Params p, int dev, cudaStream_t st) {
+  const int64_t want = (int64_t)p.rows * p.V / ((int64_t)g_dev[dev].sms * 4);
+  const int64_t slice = (want + constrain::NT * 4 - 1) / (constrain::NT * 4) * (constrain::NT * 4);
+  p.slice = (int)(slice < constrain::NT * 4 ? constrain::NT * 4 : slice > constrain::SLICE ? constrain::SLICE : slice);
+  const dim3 grid((p.V + p.slice - 1) / p.slice, p.rows);
+  const size_t smem = p.T > 0 ? (size_t)p.slice * 4 : 0;
+  const bool vec = p.V % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0;
+  const int slot = kSlotConstrain + (sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2);
+  int rc = set_smem(dev, slot, constrain::constrain_kernel<T, true>, constrain::SLICE * 4);
+  if (!rc) rc = set_smem(dev, slot + 3, constrain::constrain_kernel<T, false>, constrain::SLICE * 4);
+  if (rc) return rc;
+  return vec ? launch_pdl(constrain::constrain_kernel<T, true>, grid, constrain::NT, smem, st, p)
+             : launch_pdl(constrain::constrain_kernel<T, false>, grid, constrain::NT, smem, st, p);
 }
 
 int constrain_logits(const constrain::Params& p, int dt, cudaStream_t st) {
@@ -1353,10 +1402,9 @@ int constrain_logits(const constrain::Params& p, int dt, cudaStream_t st) {
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  const dim3 grid((p.V + constrain::SLICE - 1) / constrain::SLICE, p.rows);
-  if (dt == BASAL200_BF16) return launch_pdl(constrain::constrain_kernel<__nv_bfloat16>, grid, 256, 0, st, p);
-  if (dt == BASAL200_F16) return launch_pdl(constrain::constrain_kernel<__half>, grid, 256, 0, st, p);
-  return launch_pdl(constrain::constrain_kernel<float>, grid, 256, 0, st, p);
+  if (dt == BASAL200_BF16) return constrain_launch<__nv_bfloat16>(p, dev, st);
+  if (dt == BASAL200_F16) return constrain_launch<__half>(p, dev, st);
+  return constrain_launch<float>(p, dev, st);
 }
 
 // ------------------------------------------------------------------------------------------------------------

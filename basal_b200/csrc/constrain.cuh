@@ -1,8 +1,10 @@
 // A step's logits under penalties, biases and a grammar mask, in fp32:
 //   z = logit; if the token occurs n > 0 times in the row's history: z = (z > 0 ? z / r : z r) - (f n + p);
 //   z += the biases listed for the token; z = -inf where the mask's bit is 0.
-// A token's occurrences are counted on the spot: a CTA owns a slice of the vocabulary and scans the row's history (a
-// few KB, in L2) for the tokens of its slice, so no counts are kept between steps.
+// A CTA owns a slice of a row's vocabulary. It first streams the slice (-inf where the mask's bit is 0, without reading
+// the logit; the logit elsewhere), which is all of the traffic, and then mends the few tokens that the history and the
+// biases name: the history is short beside the vocabulary, so counting its tokens of the slice in shared memory (no
+// counts are kept between steps) and rewriting those places costs less than a test at every token.
 #pragma once
 #include "quant.cuh"
 #include "paged.cuh"
@@ -10,7 +12,8 @@
 namespace b200 {
 namespace constrain {
 
-constexpr int SLICE = 2048;
+constexpr int NT = 512;         // threads
+constexpr int SLICE = 16384;    // tokens of a slice at most (4 bytes of shared memory each)
 
 struct Params {
   const void* logits;      // [rows, V], row stride ld
@@ -29,61 +32,103 @@ struct Params {
   int64_t bias_row;
   int N;
   float* out;              // [rows, V]
+  int slice;               // tokens of a slice, a multiple of 32
 };
 
 template <typename T>
 __device__ __forceinline__ float load_logit(const T* x) { return paged::widen(*x); }
 __device__ __forceinline__ float load_logit(const float* x) { return *x; }
 
-// grid (slice, row)
+// 4 consecutive logits
 template <typename T>
-__global__ void __launch_bounds__(256) constrain_kernel(const Params p) {
+__device__ __forceinline__ float4 load4(const T* x) {
+  const uint2 u = *reinterpret_cast<const uint2*>(x);
+  const T* h = reinterpret_cast<const T*>(&u);
+  return make_float4(paged::widen(h[0]), paged::widen(h[1]), paged::widen(h[2]), paged::widen(h[3]));
+}
+__device__ __forceinline__ float4 load4(const float* x) { return *reinterpret_cast<const float4*>(x); }
+
+__device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return !mask || (mask[v >> 5] >> (v & 31) & 1); }
+
+// grid (slice, row). VEC: rows of logits and of out start at multiples of 4 elements (8 or 16, and 16 bytes).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(NT) constrain_kernel(const Params p) {
+  extern __shared__ int count[];
   pdl_wait();
-  __shared__ int count[SLICE];
-  __shared__ float bias[SLICE];
-  const int b = blockIdx.y, v0 = blockIdx.x * SLICE, nv = min(SLICE, p.V - v0);
-  for (int i = threadIdx.x; i < SLICE; i += blockDim.x) {
-    count[i] = 0;
-    bias[i] = 0.0f;
+  pdl_launch();
+  const int b = blockIdx.y, v0 = blockIdx.x * p.slice, nv = min(p.slice, p.V - v0);
+  const T* z = static_cast<const T*>(p.logits) + b * p.ld + v0;
+  const uint32_t* mask = p.mask ? p.mask + b * p.mask_row + (v0 >> 5) : nullptr;
+  float* out = p.out + (int64_t)b * p.V + v0;
+
+  if (p.T > 0)
+    for (int i = threadIdx.x; i < p.slice / 4; i += NT) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
+  if constexpr (VEC) {
+#pragma unroll 4
+    for (int i = threadIdx.x * 4; i < nv; i += NT * 4) {
+      const uint32_t m = mask ? mask[i >> 5] >> (i & 31) & 15u : 15u;
+      float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (i + 4 <= nv) {
+        if (m) {
+          const float4 x = load4(z + i);
+          y.x = m & 1 ? x.x : y.x;
+          y.y = m & 2 ? x.y : y.y;
+          y.z = m & 4 ? x.z : y.z;
+          y.w = m & 8 ? x.w : y.w;
+        }
+        *reinterpret_cast<float4*>(out + i) = y;
+      } else {
+        for (int j = 0; i + j < nv; ++j) out[i + j] = m >> j & 1 ? load_logit(z + i + j) : -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < nv; i += NT) out[i] = allowed(mask, i) ? load_logit(z + i) : -INFINITY;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.T; i += blockDim.x) {
-    const int id = p.past[b * p.past_row + i];
-    if (id >= v0 && id - v0 < nv) atomicAdd(&count[id - v0], 1);
-    if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
-  }
-  // a token listed more than once gets its values in the list's order: the first of its places adds them all
-  const int32_t* ids = p.ids + b * p.bias_row;
-  for (int i = threadIdx.x; i < p.N; i += blockDim.x) {
-    const int id = ids[i];
-    if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
-    if (id >= v0 && id - v0 < nv) {
-      bool first = true;
-      for (int j = 0; j < i; ++j) first &= ids[j] != id;
-      if (first) {
-        float s = 0.0f;
-        for (int j = i; j < p.N; ++j)
-          if (ids[j] == id) s = __fadd_rn(s, p.values[b * p.bias_row + j]);
-        bias[id - v0] = s;
+
+  if (p.T > 0) {
+    const int32_t* past = p.past + b * p.past_row;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.T; i += NT) {
+      const int id = past[i];
+      if (id >= v0 && id - v0 < nv) atomicAdd(&count[id - v0], 1);
+      if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
+    }
+    __syncthreads();
+    const float r = p.repetition ? p.repetition[b] : 1.0f, pr = p.presence ? p.presence[b] : 0.0f,
+                f = p.frequency ? p.frequency[b] : 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.T; i += NT) {
+      const int v = past[i] - v0;  // negative ids stay negative
+      if (v >= 0 && v < nv && allowed(mask, v)) {
+        const int n = atomicExch(&count[v], 0);  // whoever takes the count mends the place
+        if (n > 0) {
+          const float x = load_logit(z + v);
+          out[v] = __fsub_rn(x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r), __fadd_rn(__fmul_rn(f, (float)n), pr));
+        }
       }
     }
   }
-  __syncthreads();
-  const float r = p.repetition ? p.repetition[b] : 1.0f, pr = p.presence ? p.presence[b] : 0.0f,
-              f = p.frequency ? p.frequency[b] : 0.0f;
-  for (int i = threadIdx.x; i < nv; i += blockDim.x) {
-    const int v = v0 + i;
-    float z = -INFINITY;
-    if (!p.mask || (p.mask[b * p.mask_row + (v >> 5)] >> (v & 31) & 1)) {
-      z = load_logit(static_cast<const T*>(p.logits) + b * p.ld + v);
-      const int n = count[i];
-      if (n > 0)
-        z = __fsub_rn(z > 0.0f ? __fdiv_rn(z, r) : __fmul_rn(z, r), __fadd_rn(__fmul_rn(f, (float)n), pr));
-      z = __fadd_rn(z, bias[i]);
+  if (p.N > 0) {
+    __syncthreads();
+    const int32_t* ids = p.ids + b * p.bias_row;
+    for (int i = threadIdx.x; i < p.N; i += NT) {
+      const int id = ids[i];
+      if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
+      if (id >= v0 && id - v0 < nv && allowed(mask, id - v0)) {
+        // a token listed more than once gets its values in the list's order: the first of its places adds them all
+        bool first = true;
+        for (int j = 0; j < i; ++j) first &= ids[j] != id;
+        if (first) {
+          float y = out[id - v0];
+          for (int j = i; j < p.N; ++j)
+            if (ids[j] == id) y = __fadd_rn(y, p.values[b * p.bias_row + j]);
+          out[id - v0] = y;
+        }
+      }
     }
-    p.out[(int64_t)b * p.V + v] = z;
   }
-  pdl_launch();
 }
 
 }  // namespace constrain

@@ -2,7 +2,15 @@
 // 4-tap convolution and SiLU rounded to 16 bits, l2 norms, gates) and the gated delta rule's single-token form, with
 // the row's state S [128, 128] (fp32) and last 3 convolution inputs updated in place:
 //   S' = e^g S + k (beta (v - e^g S^T k))^T,  o = S'^T q.
-// The work is the state's traffic (128 KB read and written a row and value head, 7 operations an element).
+// The work is the state's traffic: 128 KB read and written a row and value head, 7 operations an element, so the state
+// is read once into registers (all of a thread's loads are issued before the input steps, which run while they
+// arrive), updated there and written once.
+//
+// A column of S depends on the others only through k and q, so a (row, key head) is split over 1 or 8 CTAs by columns:
+// one of 128 columns where the rows fill the GPU, a cluster of 8 of 16 columns where they do not. The CTAs of a
+// cluster all read the key head's convolution inputs, so the new ones are written after a barrier of the cluster. A
+// column's sums over the 128 rows of S are the same binary tree over 32 groups of 4 rows in either form: a row's bits
+// do not depend on how many rows the call has.
 #pragma once
 #include "hybrid.cuh"
 
@@ -39,76 +47,152 @@ __device__ __forceinline__ int row_slot(const Params& p, int b, int64_t* slot) {
   return mine < 0 ? 0 : (mine < p.slots ? 1 : -1);
 }
 
-// The convolution + SiLU of channel c for the row's token, rounded to T (conv4_tokens' arithmetic).
+// The convolution + SiLU of channels c .. c + 3 for the row's token, each rounded to T (conv4_tokens' arithmetic).
 template <typename T>
-__device__ __forceinline__ float conv_channel(const T* x, const T* tail, const T* conv, int C, int c) {
-  using hybrid::to_f;
-  float acc = __fmul_rn(to_f<T>(tail[c]), to_f<T>(conv[(int64_t)c * 4]));
-  acc = __fadd_rn(acc, __fmul_rn(to_f<T>(tail[C + c]), to_f<T>(conv[(int64_t)c * 4 + 1])));
-  acc = __fadd_rn(acc, __fmul_rn(to_f<T>(tail[2 * C + c]), to_f<T>(conv[(int64_t)c * 4 + 2])));
-  acc = __fadd_rn(acc, __fmul_rn(to_f<T>(x[c]), to_f<T>(conv[(int64_t)c * 4 + 3])));
-  return hybrid::round_to<T>(hybrid::silu_f(acc));
+__device__ __forceinline__ void conv4(const T* x, const T* tail, const T* conv, int C, int c, float (&y)[4]) {
+  float in[4][4], w[4][4];
+#pragma unroll
+  for (int j = 0; j < 3; ++j) hybrid::ld4(tail + (int64_t)j * C + c, in[j]);
+  hybrid::ld4(x + c, in[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) hybrid::ld4(conv + (int64_t)(c + i) * 4, w[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float acc = __fmul_rn(in[0][i], w[i][0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) acc = __fadd_rn(acc, __fmul_rn(in[j][i], w[i][j]));
+    y[i] = hybrid::round_to<T>(hybrid::silu_f(acc));
+  }
 }
 
-// A CTA of 128 threads per (key head, row), its value heads one after another; thread j owns column j of the state.
-template <typename T>
-__global__ void __launch_bounds__(128) gdn_step_kernel(const Params p) {
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+__device__ __forceinline__ float4 fma4(float s, float4 a, float4 b) {
+  return make_float4(fmaf(s, a.x, b.x), fmaf(s, a.y, b.y), fmaf(s, a.z, b.z), fmaf(s, a.w, b.w));
+}
+
+// The sum of N values `stride` apart as a binary tree.
+template <int N>
+__device__ __forceinline__ float4 tree(const float4* v, int stride) {
+  if constexpr (N == 1)
+    return *v;
+  else
+    return add4(tree<N / 2>(v, stride), tree<N / 2>(v + N / 2 * stride, stride));
+}
+
+// CB columns a CTA, NT threads: CB / 4 lanes of 4 columns by NT / (CB / 4) bands of rows. Grid (Hk * 128 / CB, rows),
+// clusters of 128 / CB.
+template <typename T, int CB, int NT>
+__global__ void __launch_bounds__(NT) gdn_step_kernel(const Params p) {
+  constexpr int LANES = CB / 4, BANDS = NT / LANES, ROWS = 128 / BANDS, SPLIT = 128 / CB;
+  constexpr int GROUPS = ROWS / 4;  // groups of 4 rows a thread
+  static_assert(ROWS % 4 == 0 && NT % 32 == 0, "bands of whole groups");
+  __shared__ float sq[128], sk[128];
+  __shared__ __align__(16) float4 part[BANDS][LANES];
   pdl_wait();
-  const int h = blockIdx.x, b = blockIdx.y, j = threadIdx.x, rep = p.Hv / p.Hk;
+  pdl_launch();
+  const int h = blockIdx.x / SPLIT, cb = blockIdx.x % SPLIT, b = blockIdx.y, rep = p.Hv / p.Hk;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int band = threadIdx.x / LANES, col = cb * CB + threadIdx.x % LANES * 4;
   const int C = (2 * p.Hk + p.Hv) * 128;
   T* out = static_cast<T*>(p.o) + ((int64_t)b * p.Hv + h * rep) * 128;
   int64_t slot;
   const int ok = row_slot(p, b, &slot);
-  if (ok <= 0) {
-    if (ok < 0 && j == 0) atomicOr(&g_fault, (unsigned)kFaultBadSlot);
-    for (int r = 0; r < rep; ++r) out[r * 128 + j] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
-  } else {
-    const T* x = static_cast<const T*>(p.proj) + b * p.ld;
-    T* tail = static_cast<T*>(p.tail) + slot * 3 * C;
-    const T* conv = static_cast<const T*>(p.conv);
-    __shared__ float sq[128], sk[128], part[2][4];
-    const int cq = h * 128 + j, ck = p.Hk * 128 + cq;
-    const float yq = conv_channel(x, tail, conv, C, cq), yk = conv_channel(x, tail, conv, C, ck);
-    const float ssq = hybrid::warp_sum(__fmul_rn(yq, yq)), ssk = hybrid::warp_sum(__fmul_rn(yk, yk));
-    if ((j & 31) == 0) {
-      part[0][j >> 5] = ssq;
-      part[1][j >> 5] = ssk;
-    }
-    __syncthreads();
-    const float nq = rsqrtf((part[0][0] + part[0][1]) + (part[0][2] + part[0][3]) + 1e-6f);
-    const float nk = rsqrtf((part[1][0] + part[1][1]) + (part[1][2] + part[1][3]) + 1e-6f);
-    sq[j] = __fmul_rn(__fmul_rn(yq, nq), p.q_scale);
-    sk[j] = __fmul_rn(yk, nk);
-    __syncthreads();
-    for (int r = 0; r < rep; ++r) {
-      const int vh = h * rep + r, cv = 2 * p.Hk * 128 + vh * 128 + j;
-      const float v = conv_channel(x, tail, conv, C, cv);
-      const float beta = hybrid::round_to<T>(hybrid::sigmoid_f(hybrid::to_f<T>(x[p.b_off + vh])));
-      const float dt = hybrid::to_f<T>(static_cast<const T*>(p.dt_bias)[vh]);
-      const float g = __fmul_rn(-expf(p.A_log[vh]),
-                                hybrid::softplus_f(__fadd_rn(hybrid::to_f<T>(x[p.a_off + vh]), dt)));
-      const float decay = expf(g);
-      float* S = p.state + (slot * p.Hv + vh) * 16384 + j;
-      float kv = 0.0f;
-      for (int i = 0; i < 128; ++i) kv = fmaf(sk[i], decay * S[i * 128], kv);
-      const float u = beta * (v - kv);
-      float o = 0.0f;
-      for (int i = 0; i < 128; ++i) {
-        const float s = fmaf(sk[i], u, decay * S[i * 128]);
-        S[i * 128] = s;
-        o = fmaf(sq[i], s, o);
-      }
-      out[r * 128 + j] = hybrid::from_f<T>(o);
-    }
-    // the convolution's last inputs: every thread moves the channels that it alone read
-    for (int r = 0; r < 2 + rep; ++r) {
-      const int c = r == 0 ? cq : r == 1 ? ck : 2 * p.Hk * 128 + (h * rep + r - 2) * 128 + j;
-      tail[c] = tail[C + c];
-      tail[C + c] = tail[2 * C + c];
-      tail[2 * C + c] = x[c];
-    }
+  if (ok <= 0) {  // uniform over the cluster
+    if (ok < 0 && threadIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadSlot);
+    for (int i = threadIdx.x; i < rep * CB; i += NT)
+      out[i / CB * 128 + cb * CB + i % CB] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
+    return;
   }
-  pdl_launch();
+  const T* x = static_cast<const T*>(p.proj) + b * p.ld;
+  T* tail = static_cast<T*>(p.tail) + slot * 3 * C;
+  const T* conv = static_cast<const T*>(p.conv);
+  float4* S = reinterpret_cast<float4*>(p.state + ((slot * p.Hv + h * rep) * 128 + band * ROWS) * 128 + col);
+  float4 s[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
+
+  // q and k of the key head: a warp each, 4 channels a lane
+  for (int t = warp; t < 2; t += NT / 32) {
+    float y[4];
+    conv4(x, tail, conv, C, t * p.Hk * 128 + h * 128 + lane * 4, y);
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = __fadd_rn(ss, __fmul_rn(y[i], y[i]));
+    const float rn = rsqrtf(__fadd_rn(hybrid::warp_sum(ss), 1e-6f));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      (t == 0 ? sq : sk)[lane * 4 + i] = t == 0 ? __fmul_rn(__fmul_rn(y[i], rn), p.q_scale) : __fmul_rn(y[i], rn);
+  }
+  __syncthreads();
+
+  for (int r = 0; r < rep; ++r) {
+    const int vh = h * rep + r;
+    float v[4];
+    conv4(x, tail, conv, C, 2 * p.Hk * 128 + vh * 128 + col, v);  // the same in every band
+    const float beta = hybrid::round_to<T>(hybrid::sigmoid_f(hybrid::to_f<T>(x[p.b_off + vh])));
+    const float dt = hybrid::to_f<T>(static_cast<const T*>(p.dt_bias)[vh]);
+    const float g =
+        __fmul_rn(-expf(p.A_log[vh]), hybrid::softplus_f(__fadd_rn(hybrid::to_f<T>(x[p.a_off + vh]), dt)));
+    const float decay = expf(g);
+    float4 sum[GROUPS];
+#pragma unroll
+    for (int a = 0; a < GROUPS; ++a) {
+      sum[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4& e = s[a * 4 + i];
+        e = make_float4(e.x * decay, e.y * decay, e.z * decay, e.w * decay);
+        sum[a] = fma4(sk[band * ROWS + a * 4 + i], e, sum[a]);
+      }
+    }
+    part[band][threadIdx.x % LANES] = tree<GROUPS>(sum, 1);
+    __syncthreads();
+    const float4 kv = tree<BANDS>(&part[0][threadIdx.x % LANES], LANES);
+    const float4 u = make_float4(beta * (v[0] - kv.x), beta * (v[1] - kv.y), beta * (v[2] - kv.z),
+                                 beta * (v[3] - kv.w));
+#pragma unroll
+    for (int a = 0; a < GROUPS; ++a) {
+      sum[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4& e = s[a * 4 + i];
+        e = fma4(sk[band * ROWS + a * 4 + i], u, e);
+        S[(a * 4 + i) * 32] = e;
+        sum[a] = fma4(sq[band * ROWS + a * 4 + i], e, sum[a]);
+      }
+    }
+    if (r + 1 < rep) {  // the next head's state
+      S += 128 * 32;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
+    }
+    __syncthreads();  // kv has been read
+    part[band][threadIdx.x % LANES] = tree<GROUPS>(sum, 1);
+    __syncthreads();
+    if (band == 0) {
+      const float4 o = tree<BANDS>(&part[0][threadIdx.x % LANES], LANES);
+      T y[4] = {hybrid::from_f<T>(o.x), hybrid::from_f<T>(o.y), hybrid::from_f<T>(o.z), hybrid::from_f<T>(o.w)};
+      *reinterpret_cast<uint2*>(out + r * 128 + col) = *reinterpret_cast<const uint2*>(y);
+    }
+    __syncthreads();
+  }
+
+  // the convolution's last inputs, once every CTA of the key head has read them (the loop's barriers cover this CTA)
+  if constexpr (SPLIT > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  for (int i = threadIdx.x; i < (2 + rep) * LANES; i += NT) {
+    const int which = i / LANES;
+    const int c = (which < 2 ? which * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + (h * rep + which - 2) * 128) + cb * CB +
+                  i % LANES * 4;
+    const uint2 a = *reinterpret_cast<const uint2*>(tail + C + c), d = *reinterpret_cast<const uint2*>(tail + 2 * C + c);
+    *reinterpret_cast<uint2*>(tail + c) = a;
+    *reinterpret_cast<uint2*>(tail + C + c) = d;
+    *reinterpret_cast<uint2*>(tail + 2 * C + c) = *reinterpret_cast<const uint2*>(x + c);
+  }
 }
 
 }  // namespace gdnstep

@@ -56,10 +56,13 @@ struct AttendParams {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// New tokens into the pages: a warp per (row, token, head) of the keys and of the values, a lane D / 32 consecutive
-// values. 16-bit pools take the values' bits; 8-bit pools their codes and the token's scale, by the activation
-// quantiser's arithmetic (IEEE quotients, round to nearest even, saturation).
+// New tokens into the pages: a CTA takes up to APPEND_TOKENS tokens of one row with all their heads, keys and values;
+// where each token goes is looked up once. D / 8 lanes take a token's head, 16 bytes a lane, UNROLL of them in flight.
+// 16-bit pools take the values' bits; 8-bit pools their codes and the token's scale, by the activation quantiser's
+// arithmetic (block_codes8: IEEE quotients, round to nearest even, saturation).
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int APPEND_TOKENS = 16;
+
 struct AppendParams {
   const void* src[2];      // keys, values: [rows, T, Hk, D], element strides below
   int64_t row[2], tok[2], head[2];
@@ -77,65 +80,71 @@ struct AppendParams {
   int rows, T, Hk;
 };
 
-template <int BYTES>
-struct Vec;
-template <>
-struct Vec<2> { using type = uint16_t; };
-template <>
-struct Vec<4> { using type = uint32_t; };
-template <>
-struct Vec<8> { using type = uint2; };
-template <>
-struct Vec<16> { using type = uint4; };
-
+// grid (blocks of APPEND_TOKENS tokens, rows)
 template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  constexpr int LANES = D / 8, UNROLL = 4;
+  __shared__ int64_t to[APPEND_TOKENS], scale_to[APPEND_TOKENS];  // element offsets of head 0; negative: nowhere
   pdl_wait();
-  constexpr int E = D / 32;
-  using V = typename Vec<E * 2>::type;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (item < (int64_t)p.rows * p.T * p.Hk * 2) {  // warp-uniform
-    const int which = (int)(item & 1);
-    const int h = (int)((item >> 1) % p.Hk);
-    const int64_t rt = (item >> 1) / p.Hk;
-    const int t = (int)(rt % p.T), b = (int)(rt / p.T);
-    const int start = p.start[b], count = p.count ? min(p.count[b], p.T) : p.T;
-    if (start >= 0 && t < count) {
-      const int64_t pos = (int64_t)start + t;
-      const int64_t pi = pos / p.page_size;
-      const int page = pi < p.width ? p.table[b * p.table_row + pi] : -1;
-      if (page < 0 || page >= p.pages) {
-        if (lane == 0) atomicOr(&g_fault, (unsigned)kFaultBadPage);
+  pdl_launch();
+  const int b = blockIdx.y, t0 = blockIdx.x * APPEND_TOKENS;
+  const int start = p.start[b];
+  const int count = min(start < 0 ? 0 : p.count ? min(p.count[b], p.T) : p.T, t0 + APPEND_TOKENS) - t0;
+  if (count <= 0) return;  // uniform
+  if ((int)threadIdx.x < count) {
+    const int64_t pos = (int64_t)start + t0 + threadIdx.x, pi = pos / p.page_size;
+    const int off = (int)(pos - pi * p.page_size);
+    const int page = pi < p.width ? p.table[b * p.table_row + pi] : -1;
+    const bool fine = page >= 0 && page < p.pages;
+    if (!fine) atomicOr(&g_fault, (unsigned)kFaultBadPage);
+    to[threadIdx.x] = fine ? page * p.page_stride + off * p.token_stride : -1;
+    scale_to[threadIdx.x] = page * p.s_page + off;
+  }
+  __syncthreads();
+  const int l = threadIdx.x % LANES, items = count * p.Hk * 2;  // item: (token, head, keys or values)
+  constexpr int STEP = 256 / LANES;
+  const int rounds = (items + STEP * UNROLL - 1) / (STEP * UNROLL);  // the same for every thread: whole shuffles
+  for (int round = 0; round < rounds; ++round) {
+    const int first = threadIdx.x / LANES + round * STEP * UNROLL;
+    uint4 raw[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = first + u * STEP;
+      if (i < items) {
+        const int which = i & 1, h = (i >> 1) % p.Hk, t = (i >> 1) / p.Hk;
+        const T* src = static_cast<const T*>(p.src[which]) + b * p.row[which] + (t0 + t) * p.tok[which] +
+                       h * p.head[which];
+        raw[u] = *reinterpret_cast<const uint4*>(src + l * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = first + u * STEP;
+      const bool live = i < items;
+      const int which = i & 1, h = (i >> 1) % p.Hk, t = live ? (i >> 1) / p.Hk : 0;
+      const int64_t at = live ? to[t] : -1;
+      if (!FP8) {
+        if (at >= 0)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.pool[which]) + at + h * p.head_stride + l * 8) = raw[u];
       } else {
-        const int off = (int)(pos % p.page_size);
-        const T* src = static_cast<const T*>(p.src[which]) + b * p.row[which] + t * p.tok[which] + h * p.head[which];
-        const V raw = *reinterpret_cast<const V*>(src + lane * E);
-        const int64_t at = page * p.page_stride + h * p.head_stride + off * p.token_stride + lane * E;
-        if (!FP8) {
-          *reinterpret_cast<V*>(static_cast<T*>(p.pool[which]) + at) = raw;
-        } else {
-          const T* x = reinterpret_cast<const T*>(&raw);
-          float v[E], amax = 0.0f;
+        const T* x = reinterpret_cast<const T*>(&raw[u]);
+        float v[8], amax = 0.0f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            v[e] = widen(x[e]);
-            amax = max_nan(amax, fabsf(v[e]));
-          }
+        for (int e = 0; e < 8; ++e) {
+          v[e] = live ? widen(x[e]) : 0.0f;
+          amax = max_nan(amax, fabsf(v[e]));
+        }
 #pragma unroll
-          for (int o = 16; o >= 1; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          const float s = __fdiv_rn(max_nan(amax, 1e-12f), 448.0f);
-          uint8_t c[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) c[e] = float_to_e4m3(__fdiv_rn(v[e], s));
-          using W = typename std::conditional<E == 8, uint2, typename Vec<E == 8 ? 4 : E>::type>::type;
-          *reinterpret_cast<W*>(static_cast<uint8_t*>(p.pool[which]) + at) = *reinterpret_cast<const W*>(c);
-          if (lane == 0) p.scale[which][page * p.s_page + h * p.s_head + off] = s;
+        for (int o = LANES / 2; o >= 1; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float s = __fdiv_rn(max_nan(amax, 1e-12f), 448.0f);
+        const uint2 codes = block_codes8<false>(v, s);
+        if (at >= 0) {
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.pool[which]) + at + h * p.head_stride + l * 8) = codes;
+          if (l == 0) p.scale[which][scale_to[t] + h * p.s_head] = s;
         }
       }
     }
   }
-  pdl_launch();
 }
 
 // ---------------------------------------------------------------------------------------------------------------
