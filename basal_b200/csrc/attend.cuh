@@ -75,15 +75,6 @@ struct Workspace {
   int cap;   // parts_cap
 };
 
-// x / d for 0 <= x < 2^31 by a multiplication (Granlund and Montgomery 1994): shift = ceil(log2 d), mul =
-// floor(2^32 (2^shift - d) / d) + 1, x / d = (mulhi(x, mul) + x) >> shift. Exact, and the sum stays below 2^32.
-struct Divide {
-  uint32_t mul, shift;
-};
-__device__ __forceinline__ int divide(int x, Divide d) {
-  return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift);
-}
-
 // A row's span of positions, from its length: n (clamped to the table), first, and whether it was too long.
 __device__ __forceinline__ bool row_span(const AttendParams& p, int b, int* n, int* first) {
   const int len = p.lengths[b];

@@ -1161,6 +1161,12 @@ int check_cache(int dtype, int kv_dtype, int64_t page_stride, int64_t head_strid
   return BASAL200_OK;
 }
 
+paged::Divide divider(int d) {
+  uint32_t shift = 0;
+  while ((1ll << shift) < d) ++shift;
+  return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
 // Query heads that share a key / value head are taken 8 at a time (one n tile of the MMA), or 16 where there are more
 // and the accumulators fit (D <= 128).
 int attend_ng(int H, int Hk, int D) { return H / Hk > 8 && D <= 128 ? 2 : 1; }
@@ -1172,12 +1178,6 @@ int attend_parts(int64_t width, int64_t page_size, int64_t window, bool fp8, int
   const int64_t tt = paged::tile_of(fp8, D, ng), nt = (width * page_size + tt - 1) / tt, in = window / tt + 2;
   return paged::most_parts(window > 0 && in < nt ? in : nt, paged::item_tiles(fp8, D, ng),
                            paged::parts_cap(D, ng, Hk * attend_groups(H, Hk, D)));
-}
-
-paged::Divide divider(int d) {
-  uint32_t shift = 0;
-  while ((1ll << shift) < d) ++shift;
-  return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
 }
 
 template <typename TQ, bool FP8, int D, int NG>
@@ -1248,9 +1248,10 @@ int paged_attention(const paged::AttendParams& p, int q_dtype, int kv_dtype, int
 template <typename T, bool FP8>
 int append_launch(const paged::AppendParams& p, int D, cudaStream_t st) {
   const dim3 grid((p.T + paged::APPEND_TOKENS - 1) / paged::APPEND_TOKENS, p.rows);
-  if (D == 64) return launch_pdl(paged::append_kernel<T, FP8, 64>, grid, 256, 0, st, p);
-  if (D == 128) return launch_pdl(paged::append_kernel<T, FP8, 128>, grid, 256, 0, st, p);
-  return launch_pdl(paged::append_kernel<T, FP8, 256>, grid, 256, 0, st, p);
+  const paged::Divide by_head = divider(p.Hk);
+  if (D == 64) return launch_pdl(paged::append_kernel<T, FP8, 64>, grid, 256, 0, st, p, by_head);
+  if (D == 128) return launch_pdl(paged::append_kernel<T, FP8, 128>, grid, 256, 0, st, p, by_head);
+  return launch_pdl(paged::append_kernel<T, FP8, 256>, grid, 256, 0, st, p, by_head);
 }
 
 int kv_append(const paged::AppendParams& p, int dtype, int kv_dtype, int D, cudaStream_t st) {

@@ -13,6 +13,7 @@ namespace b200 {
 namespace constrain {
 
 constexpr int NT = 512;         // threads
+constexpr int HELD = 4;         // tokens of the history that a thread holds in registers
 constexpr int SLICE = 16384;    // tokens of a slice at most (4 bytes of shared memory each)
 
 struct Params {
@@ -61,54 +62,64 @@ __global__ void __launch_bounds__(NT) constrain_kernel(const Params p) {
   const uint32_t* mask = p.mask ? p.mask + b * p.mask_row + (v0 >> 5) : nullptr;
   float* out = p.out + (int64_t)b * p.V + v0;
 
+  // the history's first tokens are asked for before the slice is streamed
+  const int32_t* past = p.past + b * p.past_row;
+  int ids[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) ids[k] = (int)threadIdx.x + k * NT < p.T ? past[threadIdx.x + k * NT] : -1;
   if (p.T > 0)
     for (int i = threadIdx.x; i < p.slice / 4; i += NT) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
   if constexpr (VEC) {
-#pragma unroll 4
-    for (int i = threadIdx.x * 4; i < nv; i += NT * 4) {
-      const uint32_t m = mask ? mask[i >> 5] >> (i & 31) & 15u : 15u;
-      float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (i + 4 <= nv) {
-        if (m) {
-          const float4 x = load4(z + i);
-          y.x = m & 1 ? x.x : y.x;
-          y.y = m & 2 ? x.y : y.y;
-          y.z = m & 4 ? x.z : y.z;
-          y.w = m & 8 ? x.w : y.w;
-        }
-        *reinterpret_cast<float4*>(out + i) = y;
-      } else {
-        for (int j = 0; i + j < nv; ++j) out[i + j] = m >> j & 1 ? load_logit(z + i + j) : -INFINITY;
+    constexpr int U = 4;  // loads in flight a thread
+    int i = threadIdx.x * 4;
+    for (; i + (U - 1) * NT * 4 + 4 <= nv; i += U * NT * 4) {
+      uint32_t m[U];
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * NT * 4;
+        m[u] = mask ? mask[j >> 5] >> (j & 31) & 15u : 15u;
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = m[u] ? load4(z + i + u * NT * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        *reinterpret_cast<float4*>(out + i + u * NT * 4) =
+            make_float4(m[u] & 1 ? x[u].x : -INFINITY, m[u] & 2 ? x[u].y : -INFINITY, m[u] & 4 ? x[u].z : -INFINITY,
+                        m[u] & 8 ? x[u].w : -INFINITY);
     }
+    for (; i < nv; i += NT * 4)
+      for (int j = i; j < min(i + 4, nv); ++j) out[j] = allowed(mask, j) ? load_logit(z + j) : -INFINITY;
   } else {
 #pragma unroll 8
     for (int i = threadIdx.x; i < nv; i += NT) out[i] = allowed(mask, i) ? load_logit(z + i) : -INFINITY;
   }
 
   if (p.T > 0) {
-    const int32_t* past = p.past + b * p.past_row;
-    __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < p.T; i += NT) {
-      const int id = past[i];
+    auto tally = [&](int id) {
       if (id >= v0 && id - v0 < nv) atomicAdd(&count[id - v0], 1);
       if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
-    }
+    };
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) tally(ids[k]);
+    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) tally(past[i]);
     __syncthreads();
     const float r = p.repetition ? p.repetition[b] : 1.0f, pr = p.presence ? p.presence[b] : 0.0f,
                 f = p.frequency ? p.frequency[b] : 0.0f;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < p.T; i += NT) {
-      const int v = past[i] - v0;  // negative ids stay negative
-      if (v >= 0 && v < nv && allowed(mask, v)) {
+    auto mend = [&](int id) {
+      const int v = id - v0;
+      if (id >= v0 && v < nv && allowed(mask, v)) {
         const int n = atomicExch(&count[v], 0);  // whoever takes the count mends the place
         if (n > 0) {
           const float x = load_logit(z + v);
           out[v] = __fsub_rn(x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r), __fadd_rn(__fmul_rn(f, (float)n), pr));
         }
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) mend(ids[k]);
+    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) mend(past[i]);
   }
   if (p.N > 0) {
     __syncthreads();

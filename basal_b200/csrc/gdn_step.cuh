@@ -84,11 +84,11 @@ __device__ __forceinline__ float4 tree(const float4* v, int stride) {
 // CB columns a CTA, NT threads: CB / 4 lanes of 4 columns by NT / (CB / 4) bands of rows. Grid (Hk * 128 / CB, rows),
 // clusters of 128 / CB.
 template <typename T, int CB, int NT>
-__global__ void __launch_bounds__(NT) gdn_step_kernel(const Params p) {
+__global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) gdn_step_kernel(const Params p) {
   constexpr int LANES = CB / 4, BANDS = NT / LANES, ROWS = 128 / BANDS, SPLIT = 128 / CB;
   constexpr int GROUPS = ROWS / 4;  // groups of 4 rows a thread
   static_assert(ROWS % 4 == 0 && NT % 32 == 0, "bands of whole groups");
-  __shared__ float sq[128], sk[128];
+  __shared__ __align__(16) float sq[128], sk[128];
   __shared__ __align__(16) float4 part[BANDS][LANES];
   pdl_wait();
   pdl_launch();
@@ -140,11 +140,13 @@ __global__ void __launch_bounds__(NT) gdn_step_kernel(const Params p) {
 #pragma unroll
     for (int a = 0; a < GROUPS; ++a) {
       sum[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 k4 = *reinterpret_cast<const float4*>(&sk[band * ROWS + a * 4]);
+      const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float4& e = s[a * 4 + i];
         e = make_float4(e.x * decay, e.y * decay, e.z * decay, e.w * decay);
-        sum[a] = fma4(sk[band * ROWS + a * 4 + i], e, sum[a]);
+        sum[a] = fma4(kk[i], e, sum[a]);
       }
     }
     part[band][threadIdx.x % LANES] = tree<GROUPS>(sum, 1);
@@ -155,12 +157,15 @@ __global__ void __launch_bounds__(NT) gdn_step_kernel(const Params p) {
 #pragma unroll
     for (int a = 0; a < GROUPS; ++a) {
       sum[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 k4 = *reinterpret_cast<const float4*>(&sk[band * ROWS + a * 4]);
+      const float4 q4 = *reinterpret_cast<const float4*>(&sq[band * ROWS + a * 4]);
+      const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, qq[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float4& e = s[a * 4 + i];
-        e = fma4(sk[band * ROWS + a * 4 + i], u, e);
+        e = fma4(kk[i], u, e);
         S[(a * 4 + i) * 32] = e;
-        sum[a] = fma4(sq[band * ROWS + a * 4 + i], e, sum[a]);
+        sum[a] = fma4(qq[i], e, sum[a]);
       }
     }
     if (r + 1 < rep) {  // the next head's state

@@ -34,6 +34,15 @@ __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat
 template <>
 __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 
+// x / d for 0 <= x < 2^31 by a multiplication (Granlund and Montgomery 1994): shift = ceil(log2 d), mul =
+// floor(2^32 (2^shift - d) / d) + 1, x / d = (mulhi(x, mul) + x) >> shift. Exact, and the sum stays below 2^32.
+struct Divide {
+  uint32_t mul, shift;
+};
+__device__ __forceinline__ int divide(int x, Divide d) {
+  return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift);
+}
+
 struct AttendParams {
   const void* q;           // [rows, H, D], strides q_row, q_head elements
   int64_t q_row, q_head;
@@ -82,8 +91,8 @@ struct AppendParams {
 
 // grid (blocks of APPEND_TOKENS tokens, rows)
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  constexpr int LANES = D / 8, UNROLL = 4;
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p, const Divide by_head) {
+  constexpr int LANES = D / 8, UNROLL = 2;
   __shared__ int64_t to[APPEND_TOKENS], scale_to[APPEND_TOKENS];  // element offsets of head 0; negative: nowhere
   pdl_wait();
   pdl_launch();
@@ -101,46 +110,49 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     scale_to[threadIdx.x] = page * p.s_page + off;
   }
   __syncthreads();
-  const int l = threadIdx.x % LANES, items = count * p.Hk * 2;  // item: (token, head, keys or values)
+  const int l = threadIdx.x % LANES, items = count * p.Hk;  // item: a token's head, its keys and its values
   constexpr int STEP = 256 / LANES;
   const int rounds = (items + STEP * UNROLL - 1) / (STEP * UNROLL);  // the same for every thread: whole shuffles
   for (int round = 0; round < rounds; ++round) {
-    const int first = threadIdx.x / LANES + round * STEP * UNROLL;
-    uint4 raw[UNROLL];
+    uint4 raw[UNROLL][2];
+    int64_t at[UNROLL], sat[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int i = first + u * STEP;
+      const int i = threadIdx.x / LANES + (round * UNROLL + u) * STEP;
+      at[u] = -1;
+      raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
       if (i < items) {
-        const int which = i & 1, h = (i >> 1) % p.Hk, t = (i >> 1) / p.Hk;
-        const T* src = static_cast<const T*>(p.src[which]) + b * p.row[which] + (t0 + t) * p.tok[which] +
-                       h * p.head[which];
-        raw[u] = *reinterpret_cast<const uint4*>(src + l * 8);
+        const int t = divide(i, by_head), h = i - t * p.Hk;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          raw[u][w] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.src[w]) + b * p.row[w] +
+                                                      (t0 + t) * p.tok[w] + h * p.head[w] + l * 8);
+        at[u] = to[t] < 0 ? -1 : to[t] + h * p.head_stride + l * 8;
+        sat[u] = scale_to[t] + h * p.s_head;
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int i = first + u * STEP;
-      const bool live = i < items;
-      const int which = i & 1, h = (i >> 1) % p.Hk, t = live ? (i >> 1) / p.Hk : 0;
-      const int64_t at = live ? to[t] : -1;
-      if (!FP8) {
-        if (at >= 0)
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.pool[which]) + at + h * p.head_stride + l * 8) = raw[u];
-      } else {
-        const T* x = reinterpret_cast<const T*>(&raw[u]);
-        float v[8], amax = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = live ? widen(x[e]) : 0.0f;
-          amax = max_nan(amax, fabsf(v[e]));
-        }
+      for (int w = 0; w < 2; ++w) {
+        if (!FP8) {
+          if (at[u] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.pool[w]) + at[u]) = raw[u][w];
+        } else {
+          const T* x = reinterpret_cast<const T*>(&raw[u][w]);
+          float v[8], amax = 0.0f;
 #pragma unroll
-        for (int o = LANES / 2; o >= 1; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float s = __fdiv_rn(max_nan(amax, 1e-12f), 448.0f);
-        const uint2 codes = block_codes8<false>(v, s);
-        if (at >= 0) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.pool[which]) + at + h * p.head_stride + l * 8) = codes;
-          if (l == 0) p.scale[which][scale_to[t] + h * p.s_head] = s;
+          for (int e = 0; e < 8; ++e) {
+            v[e] = widen(x[e]);
+            amax = max_nan(amax, fabsf(v[e]));
+          }
+#pragma unroll
+          for (int o = LANES / 2; o >= 1; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const float s = __fdiv_rn(max_nan(amax, 1e-12f), 448.0f);
+          const uint2 codes = block_codes8<false>(v, s);
+          if (at[u] >= 0) {
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.pool[w]) + at[u]) = codes;
+            if (l == 0) p.scale[w][sat[u]] = s;
+          }
         }
       }
     }
