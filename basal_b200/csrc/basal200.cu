@@ -51,7 +51,7 @@ enum SmemSlot {
 };
 // kSlotFp4 .. + 5, kSlotSmall .. + 11, kSlotSplit .. + 3, kSlotSplitQ .. + 7, kSlotLogits .. + 11, kSlotGlu .. + 7,
 // kSlotRes .. + 3, kSlotGdn, kSlotLogitsTc .. + 11, kSlotGdnV .. + 1, kSlotGdnVO .. + 1,
-// kSlotAttend .. + 19, kSlotConstrain .. + 5 (bits of a 128-bit mask)
+// kSlotAttend .. + 19, kSlotConstrain .. + 2 (bits of a 128-bit mask)
 
 bool smem_is_set(int dev, int slot) { return (g_dev[dev].smem_set[slot >> 6] >> (slot & 63)) & 1; }
 
@@ -146,28 +146,6 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return launched();
-  return launched();
-}
-
-// The same for a kernel whose CTAs form clusters of `cluster` along x.
-template <typename... KArgs, typename... Args>
-int launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, unsigned cluster,
-                       Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return launched();
   return launched();
 }
@@ -1343,17 +1321,6 @@ int kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_byt
   return copy_pages_launch<1024>(pools, layers, page_bytes, npools, pages, src, dst, n, st);
 }
 
-#ifndef GDN_WIDE
-#define GDN_WIDE 2
-#endif
-// A cluster of 8 CTAs of 16 columns a (row, key head) while that many CTAs of 128 columns would leave SMs idle.
-template <typename T>
-int gdn_step_launch(const gdnstep::Params& p, int dev, cudaStream_t st) {
-  if ((int64_t)p.rows * p.Hk >= GDN_WIDE * g_dev[dev].sms)
-    return launch_pdl(gdnstep::gdn_step_kernel<T, 128, 256>, dim3(p.Hk, p.rows), 256, 0, st, p);
-  return launch_pdl_cluster(gdnstep::gdn_step_kernel<T, 16, 128>, dim3(p.Hk * 8, p.rows), 128, 0, st, 8, p);
-}
-
 int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   if (p.rows < 0 || p.Hk <= 0 || p.Hv <= 0 || p.slots < 0) return BASAL200_ERR_ARG;
   if (p.Hv % p.Hk) return BASAL200_ERR_SHAPE;
@@ -1371,25 +1338,25 @@ int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  return dt == BASAL200_BF16 ? gdn_step_launch<__nv_bfloat16>(p, dev, st) : gdn_step_launch<__half>(p, dev, st);
+  const dim3 grid(p.Hk, p.rows);
+  if (dt == BASAL200_BF16) return launch_pdl(gdnstep::gdn_step_kernel<__nv_bfloat16>, grid, gdnstep::NT, 0, st, p);
+  return launch_pdl(gdnstep::gdn_step_kernel<__half>, grid, gdnstep::NT, 0, st, p);
 }
 
-// Slices of up to 16384 tokens (the history is read once a slice), smaller where few rows would leave SMs idle: about 4
-// CTAs an SM.
+// A row in equal slices: of up to 32768 tokens (the history is read once a slice), smaller where few rows would leave
+// SMs idle (about 3 CTAs an SM, but 4 tokens a thread at least).
 template <typename T>
 int constrain_launch(constrain::Params p, int dev, cudaStream_t st) {
-  const int64_t want = (int64_t)p.rows * p.V / ((int64_t)g_dev[dev].sms * 4);
-  const int64_t slice = (want + constrain::NT * 4 - 1) / (constrain::NT * 4) * (constrain::NT * 4);
-  p.slice = (int)(slice < constrain::NT * 4 ? constrain::NT * 4 : slice > constrain::SLICE ? constrain::SLICE : slice);
+  int64_t want = (int64_t)p.rows * p.V / ((int64_t)g_dev[dev].sms * 3);
+  if (want < constrain::NT * 4) want = constrain::NT * 4;
+  if (want > constrain::SLICE) want = constrain::SLICE;
+  const int64_t n = (p.V + want - 1) / want;
+  p.slice = (int)(((p.V + n - 1) / n + 31) / 32 * 32);
   const dim3 grid((p.V + p.slice - 1) / p.slice, p.rows);
-  const size_t smem = p.T > 0 ? (size_t)p.slice * 4 : 0;
-  const bool vec = p.V % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0;
   const int slot = kSlotConstrain + (sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 1 : 2);
-  int rc = set_smem(dev, slot, constrain::constrain_kernel<T, true>, constrain::SLICE * 4);
-  if (!rc) rc = set_smem(dev, slot + 3, constrain::constrain_kernel<T, false>, constrain::SLICE * 4);
+  const int rc = set_smem(dev, slot, constrain::constrain_kernel<T>, constrain::SLICE * 2);
   if (rc) return rc;
-  return vec ? launch_pdl(constrain::constrain_kernel<T, true>, grid, constrain::NT, smem, st, p)
-             : launch_pdl(constrain::constrain_kernel<T, false>, grid, constrain::NT, smem, st, p);
+  return launch_pdl(constrain::constrain_kernel<T>, grid, constrain::NT, p.T > 0 ? (size_t)p.slice * 2 : 0, st, p);
 }
 
 int constrain_logits(const constrain::Params& p, int dt, cudaStream_t st) {
@@ -1399,7 +1366,7 @@ int constrain_logits(const constrain::Params& p, int dt, cudaStream_t st) {
   if (p.rows == 0 || p.V == 0) return BASAL200_OK;
   if (!p.logits || !p.out || (p.T > 0 && !p.past) || (p.N > 0 && (!p.ids || !p.values))) return BASAL200_ERR_ARG;
   if (!aligned16(p.out)) return BASAL200_ERR_ALIGN;
-  if (p.rows > 65535 || p.V > (1 << 30) || p.N > 4096) return BASAL200_ERR_LIMIT;
+  if (p.rows > 65535 || p.V > (1 << 30) || p.N > 4096 || p.T > constrain::MAX_PAST) return BASAL200_ERR_LIMIT;
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;

@@ -12,9 +12,10 @@
 namespace b200 {
 namespace constrain {
 
-constexpr int NT = 512;         // threads
+constexpr int NT = 512;         // threads, three CTAs an SM
 constexpr int HELD = 4;         // tokens of the history that a thread holds in registers
-constexpr int SLICE = 16384;    // tokens of a slice at most (4 bytes of shared memory each)
+constexpr int SLICE = 32768;    // tokens of a slice at most: 16-bit counts, 64 KB of shared memory
+constexpr int MAX_PAST = 65535; // so that they hold
 
 struct Params {
   const void* logits;      // [rows, V], row stride ld
@@ -40,21 +41,28 @@ template <typename T>
 __device__ __forceinline__ float load_logit(const T* x) { return paged::widen(*x); }
 __device__ __forceinline__ float load_logit(const float* x) { return *x; }
 
-// 4 consecutive logits
+// 4 consecutive logits as they lie in memory, and in fp32
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* x) {
-  const uint2 u = *reinterpret_cast<const uint2*>(x);
-  const T* h = reinterpret_cast<const T*>(&u);
-  return make_float4(paged::widen(h[0]), paged::widen(h[1]), paged::widen(h[2]), paged::widen(h[3]));
-}
-__device__ __forceinline__ float4 load4(const float* x) { return *reinterpret_cast<const float4*>(x); }
+struct Four {
+  uint2 raw;
+  __device__ __forceinline__ void load(const T* x) { raw = *reinterpret_cast<const uint2*>(x); }
+  __device__ __forceinline__ void zero() { raw = make_uint2(0, 0); }
+  __device__ __forceinline__ float get(int i) const { return paged::widen(reinterpret_cast<const T*>(&raw)[i]); }
+};
+template <>
+struct Four<float> {
+  float4 raw;
+  __device__ __forceinline__ void load(const float* x) { raw = *reinterpret_cast<const float4*>(x); }
+  __device__ __forceinline__ void zero() { raw = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  __device__ __forceinline__ float get(int i) const { return reinterpret_cast<const float*>(&raw)[i]; }
+};
 
 __device__ __forceinline__ bool allowed(const uint32_t* mask, int v) { return !mask || (mask[v >> 5] >> (v & 31) & 1); }
 
-// grid (slice, row). VEC: rows of logits and of out start at multiples of 4 elements (8 or 16, and 16 bytes).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(NT) constrain_kernel(const Params p) {
-  extern __shared__ int count[];
+// grid (slice, row)
+template <typename T>
+__global__ void __launch_bounds__(NT, 3) constrain_kernel(const Params p) {
+  extern __shared__ uint32_t count[];  // two tokens a word
   pdl_wait();
   pdl_launch();
   const int b = blockIdx.y, v0 = blockIdx.x * p.slice, nv = min(p.slice, p.V - v0);
@@ -62,70 +70,105 @@ __global__ void __launch_bounds__(NT) constrain_kernel(const Params p) {
   const uint32_t* mask = p.mask ? p.mask + b * p.mask_row + (v0 >> 5) : nullptr;
   float* out = p.out + (int64_t)b * p.V + v0;
 
-  // the history's first tokens are asked for before the slice is streamed
   const int32_t* past = p.past + b * p.past_row;
-  int ids[HELD];
+  const int32_t* ids = p.ids + b * p.bias_row;
+  const float* values = p.values + b * p.bias_row;
+  const int bias_id = (int)threadIdx.x < p.N ? ids[threadIdx.x] : -1;
+
+  // What the history makes of its tokens: counted before the slice is streamed, and for the first HELD * NT places the
+  // new value too, so that only stores are left for afterwards.
+  int held[HELD];
+  float made[HELD];
+  const float rep = p.T > 0 && p.repetition ? p.repetition[b] : 1.0f, pr = p.T > 0 && p.presence ? p.presence[b] : 0.0f,
+              fr = p.T > 0 && p.frequency ? p.frequency[b] : 0.0f;
+  auto take = [&](int id) {  // the token's count, given to one caller; 0 to the others and where there is nothing to do
+    const int v = id - v0;
+    if (id < v0 || v >= nv || !allowed(mask, v)) return 0;
+    const int at = (v & 1) * 16;
+    return (int)(atomicAnd(&count[v >> 1], ~(0xFFFFu << at)) >> at & 0xFFFFu);
+  };
+  auto penal = [&](int id, int n) {
+    const float x = load_logit(z + id - v0);
+    return __fsub_rn(x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep), __fadd_rn(__fmul_rn(fr, (float)n), pr));
+  };
+  if (p.T > 0) {
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) ids[k] = (int)threadIdx.x + k * NT < p.T ? past[threadIdx.x + k * NT] : -1;
-  if (p.T > 0)
-    for (int i = threadIdx.x; i < p.slice / 4; i += NT) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
-  if constexpr (VEC) {
+    for (int k = 0; k < HELD; ++k) held[k] = (int)threadIdx.x + k * NT < p.T ? past[threadIdx.x + k * NT] : -1;
+    for (int i = threadIdx.x; i < p.slice / 8; i += NT) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    auto tally = [&](int id) {
+      if (id >= v0 && id - v0 < nv) atomicAdd(&count[(id - v0) >> 1], 1u << ((id - v0) & 1) * 16);
+      if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) tally(held[k]);
+    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) tally(past[i]);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int n = take(held[k]);
+      made[k] = n > 0 ? penal(held[k], n) : 0.0f;
+      if (n <= 0) held[k] = -1;
+    }
+  }
+
+  // The slice in groups of 4 from the first one whose stores are 16-byte aligned (rows of any V), where the logits'
+  // groups are aligned too.
+  const int head = min((int)(-(reinterpret_cast<intptr_t>(out) >> 2) & 3), nv);
+  if (reinterpret_cast<uintptr_t>(z + head) % (4 * sizeof(T)) == 0) {
     constexpr int U = 4;  // loads in flight a thread
-    int i = threadIdx.x * 4;
+    if ((int)threadIdx.x < head)
+      out[threadIdx.x] = allowed(mask, threadIdx.x) ? load_logit(z + threadIdx.x) : -INFINITY;
+    auto four = [&](int i) -> uint32_t {  // the mask's bits i .. i + 3
+      if (!mask) return 15u;
+      const uint32_t lo = mask[i >> 5], hi = (i & 31) > 28 ? mask[(i >> 5) + 1] : 0u;
+      return __funnelshift_r(lo, hi, i & 31) & 15u;
+    };
+    int i = head + threadIdx.x * 4;
     for (; i + (U - 1) * NT * 4 + 4 <= nv; i += U * NT * 4) {
       uint32_t m[U];
-      float4 x[U];
+      Four<T> x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) m[u] = four(i + u * NT * 4);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = i + u * NT * 4;
-        m[u] = mask ? mask[j >> 5] >> (j & 31) & 15u : 15u;
+        x[u].zero();
+        if (m[u]) x[u].load(z + i + u * NT * 4);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = m[u] ? load4(z + i + u * NT * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int u = 0; u < U; ++u)
         *reinterpret_cast<float4*>(out + i + u * NT * 4) =
-            make_float4(m[u] & 1 ? x[u].x : -INFINITY, m[u] & 2 ? x[u].y : -INFINITY, m[u] & 4 ? x[u].z : -INFINITY,
-                        m[u] & 8 ? x[u].w : -INFINITY);
+            make_float4(m[u] & 1 ? x[u].get(0) : -INFINITY, m[u] & 2 ? x[u].get(1) : -INFINITY,
+                        m[u] & 4 ? x[u].get(2) : -INFINITY, m[u] & 8 ? x[u].get(3) : -INFINITY);
     }
-    for (; i < nv; i += NT * 4)
-      for (int j = i; j < min(i + 4, nv); ++j) out[j] = allowed(mask, j) ? load_logit(z + j) : -INFINITY;
+    for (; i + 4 <= nv; i += NT * 4) {
+      const uint32_t m = four(i);
+      Four<T> x;
+      x.zero();
+      if (m) x.load(z + i);
+      *reinterpret_cast<float4*>(out + i) = make_float4(m & 1 ? x.get(0) : -INFINITY, m & 2 ? x.get(1) : -INFINITY,
+                                                        m & 4 ? x.get(2) : -INFINITY, m & 8 ? x.get(3) : -INFINITY);
+    }
+    for (int j = i; j < nv && j < i + 4; ++j) out[j] = allowed(mask, j) ? load_logit(z + j) : -INFINITY;
   } else {
 #pragma unroll 8
     for (int i = threadIdx.x; i < nv; i += NT) out[i] = allowed(mask, i) ? load_logit(z + i) : -INFINITY;
   }
 
   if (p.T > 0) {
-    auto tally = [&](int id) {
-      if (id >= v0 && id - v0 < nv) atomicAdd(&count[id - v0], 1);
-      if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
-    };
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) tally(ids[k]);
-    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) tally(past[i]);
-    __syncthreads();
-    const float r = p.repetition ? p.repetition[b] : 1.0f, pr = p.presence ? p.presence[b] : 0.0f,
-                f = p.frequency ? p.frequency[b] : 0.0f;
-    auto mend = [&](int id) {
-      const int v = id - v0;
-      if (id >= v0 && v < nv && allowed(mask, v)) {
-        const int n = atomicExch(&count[v], 0);  // whoever takes the count mends the place
-        if (n > 0) {
-          const float x = load_logit(z + v);
-          out[v] = __fsub_rn(x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r), __fadd_rn(__fmul_rn(f, (float)n), pr));
-        }
-      }
-    };
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) mend(ids[k]);
-    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) mend(past[i]);
+    for (int k = 0; k < HELD; ++k)
+      if (held[k] >= 0) out[held[k] - v0] = made[k];
+    for (int i = threadIdx.x + HELD * NT; i < p.T; i += NT) {
+      const int id = past[i], n = take(id);
+      if (n > 0) out[id - v0] = penal(id, n);
+    }
   }
   if (p.N > 0) {
     __syncthreads();
-    const int32_t* ids = p.ids + b * p.bias_row;
     for (int i = threadIdx.x; i < p.N; i += NT) {
-      const int id = ids[i];
+      const int id = i < NT ? bias_id : ids[i];
       if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
       if (id >= v0 && id - v0 < nv && allowed(mask, id - v0)) {
         // a token listed more than once gets its values in the list's order: the first of its places adds them all
@@ -134,7 +177,7 @@ __global__ void __launch_bounds__(NT) constrain_kernel(const Params p) {
         if (first) {
           float y = out[id - v0];
           for (int j = i; j < p.N; ++j)
-            if (ids[j] == id) y = __fadd_rn(y, p.values[b * p.bias_row + j]);
+            if (ids[j] == id) y = __fadd_rn(y, values[j]);
           out[id - v0] = y;
         }
       }

@@ -3,14 +3,12 @@
 // the row's state S [128, 128] (fp32) and last 3 convolution inputs updated in place:
 //   S' = e^g S + k (beta (v - e^g S^T k))^T,  o = S'^T q.
 // The work is the state's traffic: 128 KB read and written a row and value head, 7 operations an element, so the state
-// is read once into registers (all of a thread's loads are issued before the input steps, which run while they
-// arrive), updated there and written once.
-//
-// A column of S depends on the others only through k and q, so a (row, key head) is split over 1 or 8 CTAs by columns:
-// one of 128 columns where the rows fill the GPU, a cluster of 8 of 16 columns where they do not. The CTAs of a
-// cluster all read the key head's convolution inputs, so the new ones are written after a barrier of the cluster. A
-// column's sums over the 128 rows of S are the same binary tree over 32 groups of 4 rows in either form: a row's bits
-// do not depend on how many rows the call has.
+// is read once into registers (all of a thread's loads are issued before the input steps, which run while they arrive,
+// and the next head's before the current one's output is summed), updated there and written once. A CTA of 256 threads
+// takes a row's key head and its value heads one after another (they share k and q, and the CTA alone reads and writes
+// their convolution inputs); two CTAs an SM keep 128 KB of state in flight. 256 rows of 32 heads: 174 us, 1.10 GB at
+// 6.3 TB/s (96% of a copy's rate); one row 6.8 us, its latency. Splitting a head's columns over a cluster of 8 CTAs for
+// few rows gained 0.2 us at one row and lost from 4 rows on (16 rows: 29 us against 10.9).
 #pragma once
 #include "hybrid.cuh"
 
@@ -81,28 +79,29 @@ __device__ __forceinline__ float4 tree(const float4* v, int stride) {
     return add4(tree<N / 2>(v, stride), tree<N / 2>(v + N / 2 * stride, stride));
 }
 
-// CB columns a CTA, NT threads: CB / 4 lanes of 4 columns by NT / (CB / 4) bands of rows. Grid (Hk * 128 / CB, rows),
-// clusters of 128 / CB.
-template <typename T, int CB, int NT>
-__global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) gdn_step_kernel(const Params p) {
-  constexpr int LANES = CB / 4, BANDS = NT / LANES, ROWS = 128 / BANDS, SPLIT = 128 / CB;
-  constexpr int GROUPS = ROWS / 4;  // groups of 4 rows a thread
-  static_assert(ROWS % 4 == 0 && NT % 32 == 0, "bands of whole groups");
-  __shared__ __align__(16) float sq[128], sk[128];
-  __shared__ __align__(16) float4 part[BANDS][LANES];
+constexpr int AHEAD = 6;  // value heads whose inputs are prepared at a time
+
+constexpr int NT = 256, LANES = 32, BANDS = 8, ROWS = 16;  // 32 lanes of 4 columns by 8 bands of 16 rows of S
+constexpr int GROUPS = ROWS / 4;
+
+// grid (Hk, rows). A column's sums over the rows of S are a binary tree over groups of 4 rows.
+template <typename T>
+__global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p) {
+  __shared__ __align__(16) float sq[128], sk[128], sv[AHEAD][128];
+  __shared__ float sbeta[AHEAD], sdecay[AHEAD];
+  __shared__ __align__(16) float4 part[2][BANDS][LANES];
   pdl_wait();
   pdl_launch();
-  const int h = blockIdx.x / SPLIT, cb = blockIdx.x % SPLIT, b = blockIdx.y, rep = p.Hv / p.Hk;
+  const int h = blockIdx.x, b = blockIdx.y, rep = p.Hv / p.Hk;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int band = threadIdx.x / LANES, col = cb * CB + threadIdx.x % LANES * 4;
+  const int band = threadIdx.x / LANES, mine = threadIdx.x % LANES, col = mine * 4;
   const int C = (2 * p.Hk + p.Hv) * 128;
   T* out = static_cast<T*>(p.o) + ((int64_t)b * p.Hv + h * rep) * 128;
   int64_t slot;
   const int ok = row_slot(p, b, &slot);
-  if (ok <= 0) {  // uniform over the cluster
+  if (ok <= 0) {
     if (ok < 0 && threadIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadSlot);
-    for (int i = threadIdx.x; i < rep * CB; i += NT)
-      out[i / CB * 128 + cb * CB + i % CB] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
+    for (int i = threadIdx.x; i < rep * 128; i += NT) out[i] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
     return;
   }
   const T* x = static_cast<const T*>(p.proj) + b * p.ld;
@@ -113,29 +112,36 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) gdn_step_kernel(const P
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
 
-  // q and k of the key head: a warp each, 4 channels a lane
-  for (int t = warp; t < 2; t += NT / 32) {
-    float y[4];
-    conv4(x, tail, conv, C, t * p.Hk * 128 + h * 128 + lane * 4, y);
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ss = __fadd_rn(ss, __fmul_rn(y[i], y[i]));
-    const float rn = rsqrtf(__fadd_rn(hybrid::warp_sum(ss), 1e-6f));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      (t == 0 ? sq : sk)[lane * 4 + i] = t == 0 ? __fmul_rn(__fmul_rn(y[i], rn), p.q_scale) : __fmul_rn(y[i], rn);
-  }
-  __syncthreads();
-
   for (int r = 0; r < rep; ++r) {
-    const int vh = h * rep + r;
-    float v[4];
-    conv4(x, tail, conv, C, 2 * p.Hk * 128 + vh * 128 + col, v);  // the same in every band
-    const float beta = hybrid::round_to<T>(hybrid::sigmoid_f(hybrid::to_f<T>(x[p.b_off + vh])));
-    const float dt = hybrid::to_f<T>(static_cast<const T*>(p.dt_bias)[vh]);
-    const float g =
-        __fmul_rn(-expf(p.A_log[vh]), hybrid::softplus_f(__fadd_rn(hybrid::to_f<T>(x[p.a_off + vh]), dt)));
-    const float decay = expf(g);
+    if (r % AHEAD == 0) {  // q and k (once) and the next heads' v, beta and decay: a warp each, 4 channels a lane
+      const int heads = min(AHEAD, rep - r);
+      for (int t = warp + (r ? 2 : 0); t < 2 + heads; t += NT / 32) {
+        float y[4];
+        const int vh = h * rep + r + t - 2;
+        conv4(x, tail, conv, C, (t < 2 ? t * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + vh * 128) + lane * 4, y);
+        if (t < 2) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ss = __fadd_rn(ss, __fmul_rn(y[i], y[i]));
+          const float rn = rsqrtf(__fadd_rn(hybrid::warp_sum(ss), 1e-6f));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            (t == 0 ? sq : sk)[lane * 4 + i] = t == 0 ? __fmul_rn(__fmul_rn(y[i], rn), p.q_scale) : __fmul_rn(y[i], rn);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sv[t - 2][lane * 4 + i] = y[i];
+          if (lane == 0) {
+            sbeta[t - 2] = hybrid::round_to<T>(hybrid::sigmoid_f(hybrid::to_f<T>(x[p.b_off + vh])));
+            const float dt = hybrid::to_f<T>(static_cast<const T*>(p.dt_bias)[vh]);
+            sdecay[t - 2] = expf(__fmul_rn(
+                -expf(p.A_log[vh]), hybrid::softplus_f(__fadd_rn(hybrid::to_f<T>(x[p.a_off + vh]), dt))));
+          }
+        }
+      }
+      __syncthreads();
+    }
+    const float4 v = *reinterpret_cast<const float4*>(&sv[r % AHEAD][col]);
+    const float beta = sbeta[r % AHEAD], decay = sdecay[r % AHEAD];
     float4 sum[GROUPS];
 #pragma unroll
     for (int a = 0; a < GROUPS; ++a) {
@@ -149,11 +155,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) gdn_step_kernel(const P
         sum[a] = fma4(kk[i], e, sum[a]);
       }
     }
-    part[band][threadIdx.x % LANES] = tree<GROUPS>(sum, 1);
+    part[0][band][mine] = tree<GROUPS>(sum, 1);
     __syncthreads();
-    const float4 kv = tree<BANDS>(&part[0][threadIdx.x % LANES], LANES);
-    const float4 u = make_float4(beta * (v[0] - kv.x), beta * (v[1] - kv.y), beta * (v[2] - kv.z),
-                                 beta * (v[3] - kv.w));
+    const float4 kv = tree<BANDS>(&part[0][0][mine], LANES);
+    const float4 u = make_float4(beta * (v.x - kv.x), beta * (v.y - kv.y), beta * (v.z - kv.z), beta * (v.w - kv.w));
 #pragma unroll
     for (int a = 0; a < GROUPS; ++a) {
       sum[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -173,25 +178,19 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) gdn_step_kernel(const P
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
     }
-    __syncthreads();  // kv has been read
-    part[band][threadIdx.x % LANES] = tree<GROUPS>(sum, 1);
-    __syncthreads();
+    part[1][band][mine] = tree<GROUPS>(sum, 1);
+    __syncthreads();  // also: everyone has read part[0], sv, sbeta and sdecay of this head
     if (band == 0) {
-      const float4 o = tree<BANDS>(&part[0][threadIdx.x % LANES], LANES);
+      const float4 o = tree<BANDS>(&part[1][0][mine], LANES);
       T y[4] = {hybrid::from_f<T>(o.x), hybrid::from_f<T>(o.y), hybrid::from_f<T>(o.z), hybrid::from_f<T>(o.w)};
       *reinterpret_cast<uint2*>(out + r * 128 + col) = *reinterpret_cast<const uint2*>(y);
     }
-    __syncthreads();
   }
 
-  // the convolution's last inputs, once every CTA of the key head has read them (the loop's barriers cover this CTA)
-  if constexpr (SPLIT > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
+  // the convolution's last inputs (the loop's barriers came after every read of them)
   for (int i = threadIdx.x; i < (2 + rep) * LANES; i += NT) {
     const int which = i / LANES;
-    const int c = (which < 2 ? which * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + (h * rep + which - 2) * 128) + cb * CB +
+    const int c = (which < 2 ? which * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + (h * rep + which - 2) * 128) +
                   i % LANES * 4;
     const uint2 a = *reinterpret_cast<const uint2*>(tail + C + c), d = *reinterpret_cast<const uint2*>(tail + 2 * C + c);
     *reinterpret_cast<uint2*>(tail + c) = a;

@@ -66,7 +66,8 @@ struct AttendParams {
 
 // ---------------------------------------------------------------------------------------------------------------
 // New tokens into the pages: a CTA takes up to APPEND_TOKENS tokens of one row with all their heads, keys and values;
-// where each token goes is looked up once. D / 8 lanes take a token's head, 16 bytes a lane, UNROLL of them in flight.
+// where each token goes is looked up once. D / 8 lanes (D / 16 for 8-bit
+// pages) take a token's head, its keys and its values, two of them at a time.
 // 16-bit pools take the values' bits; 8-bit pools their codes and the token's scale, by the activation quantiser's
 // arithmetic (block_codes8: IEEE quotients, round to nearest even, saturation).
 // ---------------------------------------------------------------------------------------------------------------
@@ -89,10 +90,19 @@ struct AppendParams {
   int rows, T, Hk;
 };
 
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <>
+struct Pair<__half> { using type = __half2; };
+
 // grid (blocks of APPEND_TOKENS tokens, rows)
 template <typename T, bool FP8, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p, const Divide by_head) {
-  constexpr int LANES = D / 8, UNROLL = 2;
+  // 8-bit pages: 16 values a lane, so that a token's shuffles, quotient and reciprocal serve more of them, and the codes
+  // are 16 bytes too
+  constexpr int VALUES = FP8 ? 16 : 8, LANES = D / VALUES, UNROLL = 2, WORDS = VALUES / 8;
   __shared__ int64_t to[APPEND_TOKENS], scale_to[APPEND_TOKENS];  // element offsets of head 0; negative: nowhere
   pdl_wait();
   pdl_launch();
@@ -114,20 +124,24 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p, const
   constexpr int STEP = 256 / LANES;
   const int rounds = (items + STEP * UNROLL - 1) / (STEP * UNROLL);  // the same for every thread: whole shuffles
   for (int round = 0; round < rounds; ++round) {
-    uint4 raw[UNROLL][2];
+    uint4 raw[UNROLL][2][WORDS];
     int64_t at[UNROLL], sat[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int i = threadIdx.x / LANES + (round * UNROLL + u) * STEP;
       at[u] = -1;
-      raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) raw[u][0][j] = raw[u][1][j] = make_uint4(0, 0, 0, 0);
       if (i < items) {
         const int t = divide(i, by_head), h = i - t * p.Hk;
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-          raw[u][w] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.src[w]) + b * p.row[w] +
-                                                      (t0 + t) * p.tok[w] + h * p.head[w] + l * 8);
-        at[u] = to[t] < 0 ? -1 : to[t] + h * p.head_stride + l * 8;
+        for (int w = 0; w < 2; ++w) {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.src[w]) + b * p.row[w] +
+                                                            (t0 + t) * p.tok[w] + h * p.head[w] + l * VALUES);
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) raw[u][w][j] = src[j];
+        }
+        at[u] = to[t] < 0 ? -1 : to[t] + h * p.head_stride + l * VALUES;
         sat[u] = scale_to[t] + h * p.s_head;
       }
     }
@@ -136,21 +150,29 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p, const
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         if (!FP8) {
-          if (at[u] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.pool[w]) + at[u]) = raw[u][w];
+          if (at[u] >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.pool[w]) + at[u]) = raw[u][w][0];
         } else {
-          const T* x = reinterpret_cast<const T*>(&raw[u][w]);
-          float v[8], amax = 0.0f;
+          using T2 = typename Pair<T>::type;
+          T2 top = __habs2(reinterpret_cast<const T2*>(&raw[u][w][0])[0]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] = widen(x[e]);
-            amax = max_nan(amax, fabsf(v[e]));
-          }
+          for (int j = 1; j < VALUES / 2; ++j)
+            top = __hmax2_nan(top, __habs2(reinterpret_cast<const T2*>(&raw[u][w][0])[j]));
+          float amax = max_nan(widen(top.x), widen(top.y));
 #pragma unroll
           for (int o = LANES / 2; o >= 1; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
           const float s = __fdiv_rn(max_nan(amax, 1e-12f), 448.0f);
-          const uint2 codes = block_codes8<false>(v, s);
+          uint2 codes[2];
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) {
+            const T* x = reinterpret_cast<const T*>(&raw[u][w][j]);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = widen(x[e]);
+            codes[j] = block_codes8<false>(v, s);
+          }
           if (at[u] >= 0) {
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.pool[w]) + at[u]) = codes;
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.pool[w]) + at[u]) =
+                make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
             if (l == 0) p.scale[w][sat[u]] = s;
           }
         }

@@ -889,7 +889,7 @@ def constrain_logits(logits: Tensor, mask: Optional[Tensor] = None, past: Option
                      frequency: Optional[Tensor] = None, bias_ids: Optional[Tensor] = None,
                      bias_values: Optional[Tensor] = None) -> Tensor:
     """A step's logits [rows, V] (bf16 / fp16 / fp32) under penalties, biases and a grammar mask -> fp32 [rows, V]:
-    a token that occurs n > 0 times in past [rows, T] (int32, negative entries skipped) gets z = (z > 0 ? z /
+    a token that occurs n > 0 times in past [rows, T] (int32, negative entries skipped, T <= 65535) gets z = (z > 0 ? z /
     repetition : z * repetition) - (frequency * n + presence), each fp32 [rows]; then the values listed for it in
     bias_ids (int32) / bias_values (fp32) [rows, N], N <= 4096, are added, in the list's order; then the tokens whose
     bit v % 32 of word v / 32 of mask [rows or 1, ceil(V / 32)] (int32) is 0 become -inf, whatever their logit (a row

@@ -357,7 +357,7 @@ int basal200_gdn_step(const void* proj, int dtype, int64_t ld, void* tail, const
  * repetition[b]) - (frequency[b] * n + presence[b]); then the values listed for it in ids / values [rows, N] (row
  * stride bias_row; added in the list's order where it is listed more than once) are added; then -inf where bit v % 32
  * of word v / 32 of mask [rows, ceil(V / 32)] (row stride mask_row, 0: one row for all) is 0, whatever the logit.
- * Negative ids in past and ids are skipped; one >= V is skipped and sets BASAL200_FAULT_BAD_ID. mask, past, ids,
+ * T <= 65535, N <= 4096. Negative ids in past and ids are skipped; one >= V is skipped and sets BASAL200_FAULT_BAD_ID. mask, past, ids,
  * repetition, presence and frequency may be NULL (no mask, T = 0, N = 0, 1, 0, 0). */
 int basal200_constrain_logits(const void* logits, int dtype, int64_t ld, int rows, int V, const uint32_t* mask,
                               int64_t mask_row, const int32_t* past, int64_t past_row, int T,
