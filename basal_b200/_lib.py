@@ -12,6 +12,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbasal200.so")
+TORCH_LIB_PATH = os.path.join(HERE, "libbasal200_torch.so")
 
 BF16, F16, F32, E4M3 = 0, 1, 2, 3
 DTYPE_CODE = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
@@ -88,6 +89,14 @@ def lib():
         L.basal200_device_faults.argtypes, L.basal200_device_faults.restype = [_I, _I], ctypes.c_uint
         _lib = L
     return _lib
+
+
+def load_torch_ops():
+    """Loads libbasal200_torch.so, the torch ops registered in C++ (csrc/step_ops.cpp); ImportError when it was not built."""
+    lib()
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise ImportError(f"{TORCH_LIB_PATH} is missing: build it with `python basal_b200/build.py`")
+    torch.ops.load_library(TORCH_LIB_PATH)
 
 
 def ptr(t):

@@ -1,10 +1,13 @@
-"""Builds libbasal200.so (every CUDA kernel of the package, sm_100a only) next to this file.
+"""Builds libbasal200.so (every CUDA kernel of the package, sm_100a only) and libbasal200_torch.so (the torch ops that are
+registered in C++, which call it) next to this file.
 
-    python basal_b200/build.py [--force]    (a plain script: importing basal_b200 needs the built library)
+    python basal_b200/build.py [--force]    (a plain script: importing basal_b200 needs the built libraries)
 
-nvcc cross-compiles without a GPU. The library links the CUDA runtime statically and resolves the one driver
+nvcc cross-compiles without a GPU. libbasal200.so links the CUDA runtime statically and resolves the one driver
 function it needs (cuTensorMapEncodeTiled) at run time, so it loads wherever a CUDA 12.8+ driver is present.
+libbasal200_torch.so is plain C++ against the installed torch's headers and libraries.
 """
+import importlib.util
 import os
 import subprocess
 import sys
@@ -16,21 +19,46 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", 
               "-shared", "-cudart", "static", "--expt-relaxed-constexpr"]
 
 
+TORCH_LIB = os.path.join(HERE, "libbasal200_torch.so")
+
+
 def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))) + \
         [os.path.join(os.path.dirname(HERE), "include", "basal200.h")]
 
 
-def stale():
-    if not os.path.exists(LIB):
+def torch_sources():
+    return [os.path.join(CSRC, "step_ops.cpp"), os.path.join(os.path.dirname(HERE), "include", "basal200.h")]
+
+
+def stale(lib=LIB, of=None):
+    if not os.path.exists(lib):
         return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(s) > t for s in sources())
+    t = os.path.getmtime(lib)
+    return any(os.path.getmtime(s) > t for s in of or sources())
+
+
+def build_torch(force=False):
+    """Compiles csrc/step_ops.cpp into libbasal200_torch.so, which finds libbasal200.so beside it."""
+    if not force and not stale(TORCH_LIB, torch_sources()):
+        return TORCH_LIB
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    inc = [f"-I{torch}/include", f"-I{torch}/include/torch/csrc/api/include", f"-I{cuda}/include"]
+    # the system's g++, whose libstdc++ is torch's: a compiler that links its own copy statically gives the library a
+    # second set of locales, and formatting an error's text crashes
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *inc, "-o", TORCH_LIB + ".tmp",
+                    torch_sources()[0], f"-L{torch}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", f"-L{HERE}",
+                    "-l:libbasal200.so", "-Wl,-rpath,$ORIGIN"], check=True)
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
 
 
 def build(force=False, verbose=False):
-    """Compiles csrc/basal200.cu into libbasal200.so when a source is newer than the library (or force)."""
+    """Compiles csrc/basal200.cu into libbasal200.so when a source is newer than the library (or force), then
+    libbasal200_torch.so likewise."""
     if not force and not stale():
+        build_torch()
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
     cmd = [nvcc, *NVCC_FLAGS, "-o", LIB + ".tmp", os.path.join(CSRC, "basal200.cu")]
@@ -38,6 +66,7 @@ def build(force=False, verbose=False):
         cmd.insert(1, "-Xptxas=-v")
     subprocess.run(cmd, check=True)
     os.replace(LIB + ".tmp", LIB)
+    build_torch(force)
     return LIB
 
 

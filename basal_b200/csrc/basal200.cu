@@ -1284,19 +1284,22 @@ int copy_pages_launch(void* const* pools, const int* layers, const int64_t* page
                       const int32_t* src, const int32_t* dst, int n, cudaStream_t st) {
   paged::CopyParams<N> p;
   int most = 0;
+  int64_t largest = 0;
   for (int i = 0; i < npools; ++i) {
     p.pool[i] = static_cast<char*>(pools[i]);
     p.page_bytes[i] = page_bytes[i];
     p.layer_bytes[i] = page_bytes[i] * pages;
     p.layers[i] = layers[i];
     if (layers[i] > most) most = layers[i];
+    if (page_bytes[i] > largest) largest = page_bytes[i];
   }
   if (!most) return BASAL200_OK;
+  p.chunks = (int)((largest + paged::COPY_BYTES - 1) / paged::COPY_BYTES);
   for (int at = 0; at < n; at += N) {
-    p.n = n - at < N ? n - at : N;
-    memcpy(p.src, src + at, (size_t)p.n * 4);
-    memcpy(p.dst, dst + at, (size_t)p.n * 4);
-    const int rc = launch_pdl(paged::copy_pages_kernel<N>, dim3(p.n, most, npools), 256, 0, st, p);
+    const int now = n - at < N ? n - at : N;
+    memcpy(p.src, src + at, (size_t)now * 4);
+    memcpy(p.dst, dst + at, (size_t)now * 4);
+    const int rc = launch_pdl(paged::copy_pages_kernel<N>, dim3(now * p.chunks, most, npools), 256, 0, st, p);
     if (rc) return rc;
   }
   return BASAL200_OK;
@@ -1310,7 +1313,7 @@ int kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_byt
   if (!pools || !layers || !page_bytes || !src || !dst) return BASAL200_ERR_ARG;
   for (int i = 0; i < npools; ++i) {
     if (!pools[i] || layers[i] < 0 || page_bytes[i] <= 0) return BASAL200_ERR_ARG;
-    if (layers[i] > 65535) return BASAL200_ERR_LIMIT;
+    if (layers[i] > 65535 || page_bytes[i] > ((int64_t)1 << 30)) return BASAL200_ERR_LIMIT;
     if ((reinterpret_cast<uintptr_t>(pools[i]) & 3) || page_bytes[i] % 4) return BASAL200_ERR_ALIGN;
   }
   if (!moves_are_apart(src, dst, n, pages)) return BASAL200_ERR_ARG;

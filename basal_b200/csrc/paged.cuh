@@ -193,28 +193,36 @@ struct CopyParams {
   char* pool[kCopyPools];
   int64_t layer_bytes[kCopyPools], page_bytes[kCopyPools];
   int layers[kCopyPools];
-  int n;
+  int chunks;  // CTAs of the largest page
   int32_t src[N], dst[N];
 };
 
-// grid (move, layer, pool)
+constexpr int COPY_BYTES = 16384;  // of a page, a CTA: four 16-byte loads a thread, all in flight
+
+// grid (move * chunks + chunk, layer, pool)
 template <int N>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams<N> p) {
   pdl_wait();
-  const int pool = blockIdx.z;
-  if ((int)blockIdx.y < p.layers[pool]) {
-    const int64_t bytes = p.page_bytes[pool];
-    char* base = p.pool[pool] + (int64_t)blockIdx.y * p.layer_bytes[pool];
-    const char* s = base + p.src[blockIdx.x] * bytes;
-    char* d = base + p.dst[blockIdx.x] * bytes;
-    if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)bytes) & 15) == 0)
-      for (int64_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-        *reinterpret_cast<uint4*>(d + i) = *reinterpret_cast<const uint4*>(s + i);
-    else
-      for (int64_t i = threadIdx.x * 4; i < bytes; i += blockDim.x * 4)
-        *reinterpret_cast<uint32_t*>(d + i) = *reinterpret_cast<const uint32_t*>(s + i);
-  }
   pdl_launch();
+  const int pool = blockIdx.z, move = blockIdx.x / p.chunks, chunk = blockIdx.x - move * p.chunks;
+  const int64_t bytes = p.page_bytes[pool], first = (int64_t)chunk * COPY_BYTES;
+  if ((int)blockIdx.y >= p.layers[pool] || first >= bytes) return;
+  char* base = p.pool[pool] + (int64_t)blockIdx.y * p.layer_bytes[pool];
+  const char* s = base + p.src[move] * bytes + first;
+  char* d = base + p.dst[move] * bytes + first;
+  const int n = (int)min((int64_t)COPY_BYTES, bytes - first);
+  if (((reinterpret_cast<uintptr_t>(base) | (uintptr_t)bytes) & 15) == 0) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (((int)threadIdx.x + u * 256) * 16 < n) v[u] = *reinterpret_cast<const uint4*>(s + (threadIdx.x + u * 256) * 16);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (((int)threadIdx.x + u * 256) * 16 < n) *reinterpret_cast<uint4*>(d + (threadIdx.x + u * 256) * 16) = v[u];
+  } else {
+    for (int i = threadIdx.x * 4; i < n; i += 256 * 4)
+      *reinterpret_cast<uint32_t*>(d + i) = *reinterpret_cast<const uint32_t*>(s + i);
+  }
 }
 
 }  // namespace paged

@@ -51,7 +51,6 @@ and tail), allocates its outputs (and scratch) from the caching allocator, enque
 the current stream and never synchronises: Dynamo traces them through their fake kernels and a CUDA graph captures
 their launches. They need CUDA tensors; there is no CPU implementation.
 """
-import ctypes
 from typing import Optional
 
 import torch
@@ -631,88 +630,41 @@ def _(q, k, v, g, beta, s0, o_16bit=False):
 # ---------------------------------------------------------------------------------------------------------------
 # one new token a row: the paged key / value cache, the recurrent state, the next token's logits
 # ---------------------------------------------------------------------------------------------------------------
-_STEP = torch.library.Library("basal", "FRAGMENT")
+# Registered in C++ (csrc/step_ops.cpp): a step's kernels run for a few microseconds, and so does a call from there.
+_lib.load_torch_ops()
+_STEP = torch.ops.basal
 
 
-def _step_op(schema, fake=None):
-    """Defines basal::<schema> with the decorated function as its implementation and returns the op. A step's calls
-    are short (a few microseconds of device time), so these ops are registered without torch.library.custom_op's
-    wrappers: 4 instead of 13 us of host time a call."""
-    name = schema.split("(")[0]
-
-    def wrap(f):
-        _STEP.define(schema)
-        for key in ("CUDA", "CPU"):  # CPU tensors reach the function's own checks
-            _STEP.impl(name, f, key)
-        torch.library.register_fake(f"basal::{name}", fake or (lambda *a: None), lib=_STEP)
-        return getattr(torch.ops.basal, name).default
-
-    return wrap
+@torch.library.register_fake("basal::paged_attention")
+def _(q, k_pages, v_pages, table, lengths, scale, window=0, k_scale=None, v_scale=None):
+    return q.new_empty(q.shape)
 
 
-def _on(dev, *tensors):
-    for t in tensors:
-        if t is not None and t.device != dev:
-            require_cuda(t)
-            raise ValueError(f"basal_b200: a tensor is on {t.device}, another on {dev}")
+@torch.library.register_fake("basal::kv_append")
+def _(k, v, k_pages, v_pages, table, start, count=None, k_scale=None, v_scale=None):
+    return None
 
 
-def _int32(what, t, *shape):
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{what} must be int32 {['any' if n is None else n for n in shape]}, not {t.dtype} "
-                         f"{list(t.shape)}")
-    return t
+@torch.library.register_fake("basal::kv_copy_pages")
+def _(pools, src, dst):
+    return None
 
 
-def _cache(what, k, v, ks, vs, table, rows, dtype):
-    """Checks a cache's pages, scales and table -> (pages, Hk, page size, D, dtype code, the strides' and scales'
-    arguments of the C ABI)."""
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
-        raise ValueError(f"{what}: the key and value pages must be [pages, kv heads, page size, D] alike, not "
-                         f"{list(k.shape)} and {list(v.shape)}")
-    N, Hk, ps, D = k.shape
-    if k.stride(3) != 1 and N and ps:
-        raise ValueError(f"{what}: the pages' last dimension must be contiguous")
-    fp8 = k.dtype == E4M3
-    if not fp8 and k.dtype != dtype:
-        raise ValueError(f"{what}: pages of {k.dtype} with tokens of {dtype}")
-    sp = sh = 0
-    if fp8:
-        if ks is None or vs is None or ks.shape != (N, Hk, ps) or vs.shape != ks.shape or ks.stride() != vs.stride() \
-                or ks.dtype != torch.float32 or vs.dtype != torch.float32 or (ps > 1 and ks.stride(2) != 1):
-            raise ValueError(f"{what}: 8-bit pages need fp32 scales k_scale, v_scale [{N}, {Hk}, {ps}]")
-        sp, sh, _ = ks.stride()
-    elif ks is not None or vs is not None:
-        raise ValueError(f"{what}: scales are for 8-bit pages")
-    _int32(f"{what}: the table", table, rows, None)
-    if table.shape[1] > 1 and table.stride(1) != 1:
-        raise ValueError(f"{what}: a table's rows must be contiguous")
-    return N, Hk, ps, D, _lib.E4M3 if fp8 else code(dtype), (*k.stride()[:3], ptr(ks), ptr(vs), sp, sh, N, ps,
-                                                             ptr(table), table.stride(0), table.shape[1])
+@torch.library.register_fake("basal::gdn_step")
+def _(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots=None):
+    return proj.new_empty((proj.shape[0], Hv, 1, 128))
 
 
-@_step_op("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, float scale, "
-          "int window=0, Tensor? k_scale=None, Tensor? v_scale=None) -> Tensor",
-          lambda q, *a: q.new_empty(q.shape))
-def _paged_attention(q, k_pages, v_pages, table, lengths, scale, window=0, k_scale=None, v_scale=None):
-    require_cuda(q)
-    dev = q.device
-    _on(dev, k_pages, v_pages, table, lengths, k_scale, v_scale)
-    if q.dim() != 3:
-        raise ValueError(f"paged_attention: q must be [rows, heads, D], not {list(q.shape)}")
-    rows, H, D = q.shape
-    N, Hk, ps, Dk, kvt, cache = _cache("paged_attention", k_pages, v_pages, k_scale, v_scale, table, rows, q.dtype)
-    if D != Dk or H == 0 or H % Hk:
-        raise ValueError(f"paged_attention: {H} heads of {D} over pages of {Hk} heads of {Dk}")
-    _int32("paged_attention: lengths", lengths, rows)
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-    out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
-    n = _lib.lib().basal200_paged_attention_workspace_bytes(rows, H, Hk, D, kvt, table.shape[1], ps, window)
-    work = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
-    call("basal200_paged_attention", dev, ptr(q), code(q.dtype), q.stride(0), q.stride(1), ptr(k_pages), ptr(v_pages),
-         kvt, *cache, ptr(_c(lengths)), rows, H, Hk, D, scale, window, ptr(out), ptr(work), n)
-    return out
+@torch.library.register_fake("basal::constrain_logits")
+def _(logits, mask=None, past=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias_values=None):
+    return logits.new_empty(logits.shape, dtype=torch.float32)
+
+
+_paged_attention = _STEP.paged_attention.default
+_kv_append = _STEP.kv_append.default
+_kv_copy_pages = _STEP.kv_copy_pages.default
+_gdn_step = _STEP.gdn_step.default
+_constrain_logits = _STEP.constrain_logits.default
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,
@@ -728,29 +680,6 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     return _paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)
 
 
-@_step_op("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, "
-          "Tensor? count=None, Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> ()")
-def _kv_append(k, v, k_pages, v_pages, table, start, count=None, k_scale=None, v_scale=None):
-    require_cuda(k)
-    dev = k.device
-    _on(dev, v, k_pages, v_pages, table, start, count, k_scale, v_scale)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"kv_append: k and v must be [rows, tokens, kv heads, D] alike, not {list(k.shape)} and "
-                         f"{list(v.shape)}")
-    rows, T, h, d = k.shape
-    N, Hk, ps, D, kvt, cache = _cache("kv_append", k_pages, v_pages, k_scale, v_scale, table, rows, k.dtype)
-    if (h, d) != (Hk, D):
-        raise ValueError(f"kv_append: tokens of {h} heads of {d} into pages of {Hk} heads of {D}")
-    _int32("kv_append: start", start, rows)
-    if count is not None:
-        count = _c(_int32("kv_append: count", count, rows))
-    k, v = (x if x.stride(3) == 1 and not (x.stride(0) | x.stride(1) | x.stride(2)) % 8 and not x.data_ptr() % 16
-            else x.contiguous() for x in (k, v))
-    (strides, scales), rest = (cache[:3], cache[3:7]), cache[7:]
-    call("basal200_kv_append", dev, ptr(k), ptr(v), code(k.dtype), *k.stride()[:3], *v.stride()[:3], ptr(k_pages),
-         ptr(v_pages), kvt, *strides, *scales, *rest, ptr(_c(start)), ptr(count), rows, T, Hk, D)
-
-
 def kv_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, start: Tensor,
               count: Optional[Tensor] = None, k_scale: Optional[Tensor] = None,
               v_scale: Optional[Tensor] = None) -> None:
@@ -762,71 +691,12 @@ def kv_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Ten
     _kv_append(k, v, k_pages, v_pages, table, start, count, k_scale, v_scale)
 
 
-@_step_op("kv_copy_pages(Tensor(a!)[] pools, int[] src, int[] dst) -> ()")
-def _kv_copy_pages(pools, src, dst):
-    if len(src) != len(dst):
-        raise ValueError(f"kv_copy_pages: {len(src)} pages to read, {len(dst)} to write")
-    require_cuda(*pools)
-    dev, N = pools[0].device, pools[0].shape[1] if pools[0].dim() > 1 else -1
-    _on(dev, *pools)
-    for p in pools:
-        if p.dim() < 3 or p.shape[1] != N or not p.is_contiguous():
-            raise ValueError("kv_copy_pages: the pools must be contiguous [layers, pages, ...] of equally many pages")
-    if any(not 0 <= i < N for i in src) or any(not 0 <= i < N for i in dst):
-        raise ValueError(f"kv_copy_pages: a page is outside [0, {N})")
-    n, m = len(src), len(pools)
-    if n == 0 or any(p.numel() == 0 for p in pools):
-        return
-    call("basal200_kv_copy_pages", dev, (ctypes.c_void_p * m)(*(p.data_ptr() for p in pools)),
-         (ctypes.c_int * m)(*(p.shape[0] for p in pools)),
-         (ctypes.c_int64 * m)(*(p.stride(1) * p.element_size() for p in pools)), m, N, (ctypes.c_int32 * n)(*src),
-         (ctypes.c_int32 * n)(*dst), n)
-
-
 def kv_copy_pages(pools: list[Tensor], src: list[int], dst: list[int]) -> None:
     """Copies page src[i] over page dst[i] in every layer of every pool ([layers, pages, ...], contiguous; up to 8: a
     cache's keys, values and their scales). src and dst are host lists, read before the call returns; ValueError, and
     nothing copied, when a page is out of range, written twice, or both read and written."""
     if pools:  # the dispatcher goes by a tensor
         _kv_copy_pages(pools, src, dst)
-
-
-@_step_op("gdn_step(Tensor proj, Tensor(a!) tail, Tensor conv, Tensor A_log, Tensor dt_bias, Tensor(b!) state, int Hk, "
-          "int Hv, int b_off, int a_off, Tensor? slots=None) -> Tensor",
-          lambda proj, tail, conv, A_log, dt_bias, state, Hk, Hv, *a: proj.new_empty((proj.shape[0], Hv, 1, 128)))
-def _gdn_step(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots=None):
-    require_cuda(proj)
-    dev, dt = proj.device, proj.dtype
-    _on(dev, tail, conv, A_log, dt_bias, state, slots)
-    if proj.dim() != 2 or Hk <= 0 or Hv <= 0 or Hv % Hk:
-        raise ValueError(f"gdn_step: proj must be [rows, width], Hv a multiple of Hk, not {list(proj.shape)}, {Hv}, {Hk}")
-    rows, C = proj.shape[0], (2 * Hk + Hv) * 128
-    if state.dim() != 4 or state.shape[1:] != (Hv, 128, 128) or state.dtype != torch.float32 \
-            or not state.is_contiguous():
-        raise ValueError(f"gdn_step: the state must be contiguous fp32 [slots, {Hv}, 128, 128]")
-    if tail.shape != (state.shape[0], 3, C) or tail.dtype != dt or not tail.is_contiguous():
-        raise ValueError(f"gdn_step: the tail must be contiguous {dt} [{state.shape[0]}, 3, {C}]")
-    if conv.shape != (C, 4) or A_log.shape != (Hv,) or dt_bias.shape != (Hv,):
-        raise ValueError(f"gdn_step: conv must be [{C}, 4], A_log and dt_bias [{Hv}]")
-    if b_off < 0 or a_off < 0 or max(C, b_off + Hv, a_off + Hv) > proj.shape[1]:
-        raise ValueError(f"gdn_step: the projection has {proj.shape[1]} columns")
-    if slots is not None:
-        slots = _c(_int32("gdn_step: slots", slots, rows))
-    elif rows > state.shape[0]:
-        raise ValueError(f"gdn_step: {rows} rows, {state.shape[0]} states")
-    if proj.stride(1) != 1 or proj.stride(0) % 4 or proj.data_ptr() % 8:
-        proj = _aligned_rows(proj)
-    o = torch.empty((rows, Hv, 1, 128), dtype=dt, device=dev)
-    call("basal200_gdn_step", dev, ptr(proj), code(dt), proj.stride(0), ptr(tail), ptr(_c(conv.to(dt))),
-         ptr(_c(A_log.float())), ptr(_c(dt_bias.to(dt))), b_off, a_off, ptr(state), ptr(slots), state.shape[0], rows,
-         Hk, Hv, ptr(o))
-    return o
-
-
-def _aligned_rows(x):
-    """A copy of x [rows, width] whose rows start at multiples of 16 bytes."""
-    y = torch.empty((x.shape[0], x.shape[1] + -x.shape[1] % 8), dtype=x.dtype, device=x.device)[:, :x.shape[1]]
-    return y.copy_(x)
 
 
 def gdn_step(proj: Tensor, tail: Tensor, conv: Tensor, A_log: Tensor, dt_bias: Tensor, state: Tensor, Hk: int, Hv: int,
@@ -838,50 +708,6 @@ def gdn_step(proj: Tensor, tail: Tensor, conv: Tensor, A_log: Tensor, dt_bias: T
     number); negative: a row of padding, zeros, and nothing is updated. A slot that is not there, or that an earlier
     row of the call has, gives a NaN row, no update and a fault bit."""
     return _gdn_step(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots)
-
-
-@_step_op("constrain_logits(Tensor logits, Tensor? mask=None, Tensor? past=None, Tensor? repetition=None, "
-          "Tensor? presence=None, Tensor? frequency=None, Tensor? bias_ids=None, Tensor? bias_values=None) -> Tensor",
-          lambda logits, *a: logits.new_empty(logits.shape, dtype=torch.float32))
-def _constrain_logits(logits, mask=None, past=None, repetition=None, presence=None, frequency=None, bias_ids=None,
-                      bias_values=None):
-    require_cuda(logits)
-    dev = logits.device
-    _on(dev, mask, past, repetition, presence, frequency, bias_ids, bias_values)
-    if logits.dim() != 2:
-        raise ValueError(f"constrain_logits: logits must be [rows, vocabulary], not {list(logits.shape)}")
-    rows, V = logits.shape
-    if logits.stride(1) != 1 and V > 1:
-        logits = logits.contiguous()
-    rowwise = []
-    for what, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None and (t.shape != (rows,) or t.dtype != torch.float32):
-            raise ValueError(f"constrain_logits: {what} must be fp32 [{rows}], not {t.dtype} {list(t.shape)}")
-        rowwise.append(None if t is None else _c(t))
-    if past is None and any(t is not None for t in rowwise):
-        raise ValueError("constrain_logits: penalties need the rows' history (past)")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("constrain_logits: bias_ids and bias_values come together")
-    mrow = prow = brow = T = N = 0
-    if mask is not None:
-        _int32("constrain_logits: the mask", mask, None, -(-V // 32))
-        if mask.shape[0] not in (1, rows):
-            raise ValueError(f"constrain_logits: a mask of {mask.shape[0]} rows for {rows}")
-        mask = _c(mask)
-        mrow = mask.shape[1] if mask.shape[0] == rows else 0
-    if past is not None:
-        past = _c(_int32("constrain_logits: past", past, rows, None))
-        prow = T = past.shape[1]
-    if bias_ids is not None:
-        bias_ids = _c(_int32("constrain_logits: bias_ids", bias_ids, rows, None))
-        if bias_values.shape != bias_ids.shape or bias_values.dtype != torch.float32:
-            raise ValueError(f"constrain_logits: bias_values must be fp32 {list(bias_ids.shape)}")
-        bias_values = _c(bias_values)
-        brow = N = bias_ids.shape[1]
-    out = torch.empty((rows, V), dtype=torch.float32, device=dev)
-    call("basal200_constrain_logits", dev, ptr(logits), code(logits.dtype), logits.stride(0), rows, V, ptr(mask), mrow,
-         ptr(past), prow, T, *map(ptr, rowwise), ptr(bias_ids), ptr(bias_values), brow, N, ptr(out))
-    return out
 
 
 def constrain_logits(logits: Tensor, mask: Optional[Tensor] = None, past: Optional[Tensor] = None,
