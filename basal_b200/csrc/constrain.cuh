@@ -73,7 +73,18 @@ __global__ void __launch_bounds__(NT, 3) constrain_kernel(const Params p) {
   const int32_t* past = p.past + b * p.past_row;
   const int32_t* ids = p.ids + b * p.bias_row;
   const float* values = p.values + b * p.bias_row;
+  // the biases' first NT places: this thread's token, whether it is of the slice and allowed, and who else names it
+  __shared__ int named[NT];
   const int bias_id = (int)threadIdx.x < p.N ? ids[threadIdx.x] : -1;
+  const float bias = (int)threadIdx.x < p.N ? values[threadIdx.x] : 0.0f;
+  bool biased = bias_id >= v0 && bias_id - v0 < nv && allowed(mask, bias_id - v0), alone = p.N <= NT;
+  if (p.N > 0) {
+    if (bias_id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
+    named[threadIdx.x] = bias_id;
+    __syncthreads();
+    if (biased)
+      for (int j = 0; j < min(p.N, NT); ++j) alone &= named[j] != bias_id || j == (int)threadIdx.x;
+  }
 
   // What the history makes of its tokens: counted before the slice is streamed, and for the first HELD * NT places the
   // new value too, so that only stores are left for afterwards.
@@ -167,15 +178,24 @@ __global__ void __launch_bounds__(NT, 3) constrain_kernel(const Params p) {
   }
   if (p.N > 0) {
     __syncthreads();
+    if (biased && alone) {
+      out[bias_id - v0] = __fadd_rn(out[bias_id - v0], bias);
+      biased = false;
+    }
+    // the others: a token listed more than once gets its values in the list's order, the first of its places adds them all
     for (int i = threadIdx.x; i < p.N; i += NT) {
       const int id = i < NT ? bias_id : ids[i];
-      if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
-      if (id >= v0 && id - v0 < nv && allowed(mask, id - v0)) {
-        // a token listed more than once gets its values in the list's order: the first of its places adds them all
+      if (i >= NT) {
+        biased = id >= v0 && id - v0 < nv && allowed(mask, id - v0);
+        if (id >= p.V && blockIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadId);
+      }
+      if (biased) {
         bool first = true;
+#pragma unroll 8
         for (int j = 0; j < i; ++j) first &= ids[j] != id;
         if (first) {
           float y = out[id - v0];
+#pragma unroll 8
           for (int j = i; j < p.N; ++j)
             if (ids[j] == id) y = __fadd_rn(y, values[j]);
           out[id - v0] = y;
