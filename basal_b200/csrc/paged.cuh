@@ -67,7 +67,7 @@ struct AttendParams {
 // ---------------------------------------------------------------------------------------------------------------
 // New tokens into the pages: a CTA takes up to APPEND_TOKENS tokens of one row with all their heads, keys and values;
 // where each token goes is looked up once. D / 8 lanes (D / 16 for 8-bit
-// pages) take a token's head, its keys and its values, two of them at a time.
+// pages) take a token's head, its keys and its values.
 // 16-bit pools take the values' bits; 8-bit pools their codes and the token's scale, by the activation quantiser's
 // arithmetic (block_codes8: IEEE quotients, round to nearest even, saturation).
 // ---------------------------------------------------------------------------------------------------------------
@@ -99,10 +99,10 @@ struct Pair<__half> { using type = __half2; };
 
 // grid (blocks of APPEND_TOKENS tokens, rows)
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p, const Divide by_head) {
+__global__ void __launch_bounds__(256, FP8 ? 5 : 1) append_kernel(const AppendParams p, const Divide by_head) {
   // 8-bit pages: 16 values a lane, so that a token's shuffles, quotient and reciprocal serve more of them, and the codes
   // are 16 bytes too
-  constexpr int VALUES = FP8 ? 16 : 8, LANES = D / VALUES, UNROLL = 2, WORDS = VALUES / 8;
+  constexpr int VALUES = FP8 ? 16 : 8, LANES = D / VALUES, UNROLL = FP8 ? 1 : 2, WORDS = VALUES / 8;
   __shared__ int64_t to[APPEND_TOKENS], scale_to[APPEND_TOKENS];  // element offsets of head 0; negative: nowhere
   pdl_wait();
   pdl_launch();
