@@ -1337,7 +1337,7 @@ int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   if (!aligned16(p.state) || !aligned16(p.conv) || !aligned16(p.o) || (p.ld % 4) ||
       (reinterpret_cast<uintptr_t>(p.proj) & 7) || (reinterpret_cast<uintptr_t>(p.tail) & 7))
     return BASAL200_ERR_ALIGN;
-  if (p.rows > 65535 || p.Hv > 65535 / 128) return BASAL200_ERR_LIMIT;
+  if (p.rows > 65535 || p.Hv > 65535) return BASAL200_ERR_LIMIT;
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
