@@ -203,12 +203,12 @@ struct AttendShape {
   static constexpr int CTAS = ctas_of(D, NG), W = warps_of(FP8, D);
   static constexpr int JHEADS = NG == 2 ? 8 : 4;        // heads that the warps join at a time, as room allows
   static constexpr int JOIN = W * JHEADS * (D + 2) * 4;
-  static constexpr int ROOM = (228 * 1024 / CTAS - 1024 - JOIN) / W;  // a warp's share
+  static constexpr int ROOM = (228 * 1024 / CTAS - 1024 - JOIN - 16) / W;  // a warp's share
   static constexpr int FIT = (ROOM - 32) / (STAGE + 32);
   static constexpr int STAGES = FIT < 6 ? FIT : 6;
   static constexpr int ITEMS = STAGES + 1;              // items that a warp may have begun to load
   static constexpr int RING = W * STAGES * STAGE;
-  static constexpr int SMEM = RING + W * ITEMS * 32 + JOIN;
+  static constexpr int SMEM = RING + W * ITEMS * 32 + JOIN + 16;
   static_assert(STAGES >= 2 && SMEM <= 227 * 1024 && (SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 
   // where a 16-byte chunk of token row `row` of a tile goes, so that the reads of a warp hit different banks
@@ -226,26 +226,38 @@ struct __align__(16) ItemInfo {
   int n, first, tile, tile_end;  // the row's span, this warp's first tile (then every W-th) and the item's end
 };
 
-// Named barriers of the joins: every warp's part is there (kBarFull), and the joining warp has read them (kBarFree + the
-// join's number % 2: the warp that joined may reach the wait after next before the others have reached the next one, and
-// must not count as one of them).
-constexpr int kBarFull = 1, kBarFree = 2;
-template <int ID, int W>
-__device__ __forceinline__ void bar_arrive() {
-  asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(W * 32) : "memory");
+// The joins' state in shared memory, counted over the kernel's life: parts left by the warps, joins read by the warps that
+// join, and whether a wait gave up. Waits are bounded (a caller that changes the lengths while the kernel reads them can
+// make its warps disagree on the items): the kernel then records a fault bit and ends.
+struct JoinState {
+  int left, read, gave_up;
+};
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.cta.shared.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+  return v;
 }
-template <int ID, int W>
-__device__ __forceinline__ void bar_wait() {
-  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(W * 32) : "memory");
+__device__ __forceinline__ void store_release(int* p, int v) {
+  asm volatile("st.release.cta.shared.s32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
 }
-// Waits until join number `join` has been read by the warp that joined it (that warp itself has nothing to wait for).
-template <int W>
-__device__ __forceinline__ void wait_joined(int join, int warp) {
-  if (join < 0 || warp == join % W) return;
-  if (join & 1)
-    bar_wait<kBarFree + 1, W>();
-  else
-    bar_wait<kBarFree, W>();
+__device__ __forceinline__ void add_release(int* p) {
+  asm volatile("red.release.cta.shared.add.s32 [%0], 1;" ::"r"(smem_u32(p)) : "memory");
+}
+// Waits until *p >= want; false when this or another warp's wait gave up. Uniform over the warp.
+__device__ __forceinline__ bool wait_for(const int* p, int want, JoinState* js) {
+  if (load_acquire(p) >= want) return true;  // lanes may differ: the vote below settles it
+  const unsigned long long t0 = globaltimer();
+  for (int n = 0;; ++n) {
+    if (load_acquire(p) >= want) return true;
+    if ((n & 255) == 255 && (load_acquire(&js->gave_up) || globaltimer() - t0 > kWaitLimitNs)) {
+      store_release(&js->gave_up, 1);
+      atomicOr(&g_fault, (unsigned)kFaultTimeoutEpilogue);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool warp_wait(const int* p, int want, JoinState* js) {
+  return __all_sync(0xffffffffu, wait_for(p, want, js));
 }
 
 template <typename TQ, bool FP8, int D, int NG>
@@ -276,6 +288,9 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
   float* join_o = reinterpret_cast<float*>(smem + Sh::RING + W * ITEMS * 32);  // [warp][JHEADS][D]
   float* join_m = join_o + W * JHEADS * D;                                     // [warp][JHEADS]
   float* join_l = join_m + W * JHEADS;
+  JoinState* js = reinterpret_cast<JoinState*>(join_l + W * JHEADS);
+  if (threadIdx.x == 0) *js = {0, 0, 0};
+  __syncthreads();
 
   pdl_wait();
   pdl_launch();  // every CTA is resident: what follows may take its place in the queue
@@ -476,12 +491,13 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
   uint32_t q[NG][QW];
   float o[NG][MT][4], mx[NG][2], sum[NG][2], fac[NG][2];  // mx: the weights' reference, base 2
   float ref_v;                                            // 8-bit: the power of two that the values' scales are over
-  int joined = 0;                                         // joins so far, of every warp
+  int joined = 0;                                         // joins so far, the same in every warp
+  bool alive = true;                                      // no wait has given up
 
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) issue(s, 0);
   int slot = 0;
-  for (int now = 0;; ++now) {
+  for (int now = 0; alive; ++now) {
     // the item's first stage (an empty one where this warp has no tile of it)
     issue(slot == 0 ? STAGES - 1 : slot - 1, now);
     cp_async_wait<STAGES - 1>();
@@ -753,9 +769,10 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
 #pragma unroll
       for (int half = 0; half < 8 / JHEADS; ++half) {
         const int live = min(JHEADS, heads - g * 8 - half * JHEADS);
-        if (live <= 0) break;
+        if (live <= 0 || !alive) break;
         const int turn = joined % W;
-        wait_joined<W>(joined - 1, warp);
+        alive = warp_wait(&js->read, joined, js);  // the last join has been read
+        if (!alive) break;
         if (JHEADS == 8 || c >> 1 == half) {
           const float back = FP8 ? ref_v : 1.0f;
 #pragma unroll
@@ -778,11 +795,12 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
             }
           }
         }
+        ++joined;
         __syncwarp();
-        if (warp != turn) {
-          bar_arrive<kBarFull, W>();
-        } else {
-          bar_wait<kBarFull, W>();
+        if (lane == 0) add_release(&js->left);
+        if (warp == turn) {
+          alive = warp_wait(&js->left, joined * W, js);
+          if (!alive) break;
 #pragma unroll 2
           for (int e = lane; e < live * (D / 4); e += 32) {
             const int head = e / (D / 4), d = e % (D / 4) * 4;
@@ -818,19 +836,14 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
             }
           }
           __syncwarp();
-          if (joined & 1)
-            bar_arrive<kBarFree + 1, W>();
-          else
-            bar_arrive<kBarFree, W>();
+          if (lane == 0) store_release(&js->read, joined);
         }
-        ++joined;
       }
     }
     if (parts < 0 && lane == 0) atomicOr(&g_fault, (unsigned)kFaultBadPage);
     __syncwarp();  // the stage and the item's entry may be filled again
     slot = slot == STAGES - 1 ? 0 : slot + 1;
   }
-  wait_joined<W>(joined - 1, warp);
   cp_async_wait<0>();
 }
 
