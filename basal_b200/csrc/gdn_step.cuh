@@ -8,7 +8,8 @@
 // takes a row's key head and its value heads one after another (they share k and q, and the CTA alone reads and writes
 // their convolution inputs); two CTAs an SM keep 128 KB of state in flight. 256 rows of 32 heads: 174 us, 1.10 GB at
 // 6.3 TB/s (96% of a copy's rate); one row 6.8 us, its latency. Splitting a head's columns over a cluster of 8 CTAs for
-// few rows gained 0.2 us at one row and lost from 4 rows on (16 rows: 29 us against 10.9).
+// few rows gained 0.2 us at one row and lost from 4 rows on (16 rows: 29 us against 10.9); a cluster of a CTA for each
+// value head gained 0.6 us up to 4 rows and lost from 8 on (256 rows: 237 us, no next head to load ahead).
 #pragma once
 #include "hybrid.cuh"
 
