@@ -435,3 +435,97 @@ def test_model_answers_under_a_grammar(ops):
         for t, v in enumerate(row):
             assert v in (1, 2) or (v // 32 == 3 + t and 0x0F0F >> v % 32 & 1)
     assert m.answer(ids, st, 0).shape == (2, 0)
+
+
+# --- as the ops are used: compiled, from threads, in one captured step ---------------------------------------------
+def decoder(ops, seed=11):
+    """A small decoding step's tensors: a cache of 3 rows (one of padding), a state pool, a history."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = inputs(3, 4, 2, 4, BF, seed)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x |= dict(k=r(9, 2, 16, 64).to(BF), v=r(9, 2, 16, 64).to(BF), q=r(3, 8, 64).to(BF), new=r(3, 1, 2, 64).to(BF),
+              table=torch.tensor([[0, 1, 2], [3, 4, -1], [-1, -1, -1]], dtype=torch.int32, device="cuda"),
+              lengths=torch.tensor([40, 17, 0], dtype=torch.int32, device="cuda"),
+              slots=torch.tensor([3, 0, -1], dtype=torch.int32, device="cuda"), logits=r(3, 500).to(BF),
+              past=torch.randint(0, 500, (3, 9), device="cuda", generator=g, dtype=torch.int32),
+              presence=torch.rand(3, device="cuda", generator=g))
+    return x
+
+
+def decode(ops, x):
+    start = x["lengths"] - 1
+    ops.kv_append(x["new"], x["new"] * 2, x["k"], x["v"], x["table"], start)
+    a = ops.paged_attention(x["q"], x["k"], x["v"], x["table"], x["lengths"], 0.125)
+    ops.kv_copy_pages([x["k"][None], x["v"][None]], [0, 3], [7, 8])
+    o = ops.gdn_step(x["proj"], x["tail"], x["conv"], x["A_log"], x["dt_bias"], x["state"], x["Hk"], x["Hv"], x["b_off"],
+                     x["a_off"], x["slots"])
+    z = ops.constrain_logits(x["logits"], None, x["past"], None, x["presence"])
+    return a, o, z
+
+
+def all_of(x, outs):
+    return [*outs, x["k"], x["v"], x["tail"], x["state"]]
+
+
+def test_a_step_compiles_as_one_graph(ops):
+    """torch.compile(fullgraph=True) of a step with all five ops: outputs and the buffers they write equal eager's."""
+    a, b = decoder(ops), decoder(ops)
+    torch._dynamo.reset()
+    f = torch.compile(lambda x: decode(ops, x), fullgraph=True)
+    for _ in range(2):
+        for got, want in zip(all_of(a, f(a)), all_of(b, decode(ops, b))):
+            assert torch.equal(got, want)
+
+
+def test_a_step_captured_and_replayed(ops):
+    """All five ops in one CUDA graph, replayed three times on inputs that changed between."""
+    a, b = decoder(ops), decoder(ops)
+    decode(ops, decoder(ops))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = decode(ops, a)
+    for n in range(3):
+        for x in (a, b):
+            x["q"].mul_(1.5)
+            x["lengths"][1] += n
+            x["past"][:, 0] = n
+        graph.replay()
+        for got, want in zip(all_of(a, outs), all_of(b, decode(ops, b))):
+            assert torch.equal(got, want), n
+
+
+def test_steps_from_two_threads(ops):
+    """Two threads, a stream each, many steps at once: each as alone."""
+    import threading
+    want = []
+    for seed in (12, 13):
+        x = decoder(ops, seed)
+        for _ in range(20):
+            outs = decode(ops, x)
+        want.append([t.clone() for t in all_of(x, outs)])
+    xs, got, streams = [decoder(ops, s) for s in (12, 13)], [None, None], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                outs = decode(ops, xs[i])
+            streams[i].synchronize()
+        got[i] = all_of(xs[i], outs)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert torch.equal(a, b)
+
+
+def test_outputs_do_not_need_gradients(ops):
+    """Inference ops: under inference_mode and no_grad alike, and queries that require gradients give none."""
+    x = decoder(ops)
+    with torch.inference_mode():
+        a = ops.paged_attention(x["q"], x["k"], x["v"], x["table"], x["lengths"], 0.125)
+    with torch.no_grad():
+        b = ops.paged_attention(x["q"].requires_grad_(), x["k"], x["v"], x["table"], x["lengths"], 0.125)
+    assert torch.equal(a, b) and not b.requires_grad
