@@ -14,7 +14,9 @@ there token by token (hybrid.HybridClassifier.open / step / answer) keeps its ke
       .free(seq)              gives its pages back
       .compact()              moves the live pages to the lowest numbers (one kv_copy_pages) -> how many pages are live
 
-The bookkeeping is on the host; the device sees the pages, and tables and lengths as int32 tensors.
+The bookkeeping is on the host; the device sees the pages, and tables and lengths as int32 tensors. A Batch says how things
+were when it was made: after grow, free or compact, make another. The copies run on the current stream: use the cache from
+one stream, or order the streams.
 """
 import dataclasses
 

@@ -674,7 +674,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     kv heads, page size, D], D = 64, 128 or 256, of q's type, or e4m3 with fp32 k_scale, v_scale [pages, kv heads, page
     size]; table [rows, width] int32: the page of positions j * page size ..; lengths [rows] int32, the new token's
     own position included (its key and value are appended first). Heads share key / value heads in order. A length <= 0
-    gives zeros. A page that is needed and not there, or a length past the table, gives a NaN row and a fault bit.
+    gives zeros. A page that is needed and not there, or a length past the table, gives a NaN row and a fault bit. What the
+    pages hold where a row reads nothing does not matter; an infinite or NaN value that it reads makes its output NaN.
     Pages may be strided views (their last dimension contiguous, the others multiples of 16 bytes). A row's output is
     the same bits alone and among other rows."""
     return _paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)
