@@ -20,6 +20,7 @@ one stream, or order the streams.
 """
 import dataclasses
 
+import numpy as np
 import torch
 
 from . import ops
@@ -57,6 +58,8 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._shares = [0] * pages   # sequences that hold a page
         self._of = {}                # sequence -> its pages, in order
+        self._row = {}               # the same as an array, made again after a change: a long cache's table is not built
+                                     # page by page at every step
         self._length = {}
         self._new = {}               # tokens that the last grow() made room for
         self._next = 0
@@ -100,6 +103,7 @@ class PagedKVCache:
             if not self._shares[p]:
                 self._free.append(p)
         del self._of[seq], self._length[seq], self._new[seq]
+        self._row.pop(seq, None)
 
     def grow(self, seqs, n=1):
         """n: tokens for each sequence, a number or a list."""
@@ -128,6 +132,7 @@ class PagedKVCache:
             self._shares[old] -= 1
             self._shares[new] = 1
             self._of[s][at] = new
+            self._row.pop(s, None)
             src.append(old)
             dst.append(new)
         if src:
@@ -135,6 +140,7 @@ class PagedKVCache:
         for s, m in zip(seqs, n):
             pages = self._of[s]
             while len(pages) * self.page_size < self._length[s] + m:
+                self._row.pop(s, None)
                 pages.append(self._free.pop())
                 self._shares[pages[-1]] = 1
             self._length[s] += m
@@ -143,13 +149,15 @@ class PagedKVCache:
     def batch(self, seqs):
         seqs = list(seqs)
         width = max([len(self._known(s)) for s in seqs], default=0) or 1
-        rows = []
-        for s in seqs:
-            rows.append(self._of[s] + [-1] * (width - len(self._of[s])) +
-                        [self._length[s], self._length[s] - self._new[s], self._new[s]])
-        host = torch.tensor(rows, dtype=torch.int32).view(len(seqs), width + 3)
-        if self.device.type == "cuda":
-            host = host.pin_memory()
+        host = torch.empty((len(seqs), width + 3), dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        rows = host.numpy()
+        for i, s in enumerate(seqs):
+            pages = self._row.get(s)
+            if pages is None:
+                pages = self._row[s] = np.asarray(self._of[s], np.int32)
+            rows[i, :len(pages)] = pages
+            rows[i, len(pages):width] = -1
+            rows[i, width:] = self._length[s], self._length[s] - self._new[s], self._new[s]
         t = host.to(self.device, non_blocking=True)
         lengths, start, count = t[:, width:].t().contiguous()
         return Batch(seqs, t[:, :width], lengths, start, count)
@@ -175,6 +183,7 @@ class PagedKVCache:
             to = dict(zip(movers, holes))
             for pages in self._of.values():
                 pages[:] = [to.get(p, p) for p in pages]
+            self._row.clear()
             for a, b in to.items():
                 self._shares[b], self._shares[a] = self._shares[a], 0
         self._free = list(range(self.pages - 1, n - 1, -1))

@@ -132,3 +132,31 @@ def test_batch(moved):
     assert got.table.tolist() == [c.pages_of(b) + [-1, -1], [-1] * 3, c.pages_of(a)]
     assert got.lengths.tolist() == [2, 0, 10] and got.start.tolist() == [0, 0, 9] and got.count.tolist() == [2, 0, 1]
     assert c.batch([]).table.shape == (0, 1)
+
+
+def test_batches_follow_every_change(moved):
+    """The table of a batch after growth, a copied page, a compaction and a freed sequence is the sequences' pages."""
+    c = cache(pages=12)
+
+    def same(*seqs):
+        got = c.batch(seqs)
+        for r, s in enumerate(seqs):
+            pages = c.pages_of(s)
+            assert got.table[r].tolist() == pages + [-1] * (got.table.shape[1] - len(pages))
+        assert got.lengths.tolist() == [c.length(s) for s in seqs]
+
+    a, b = c.add(), c.add()
+    c.grow([a, b], [6, 9])
+    same(a, b)
+    c.grow([a], 3)
+    same(b, a)
+    d = c.fork(a)
+    same(a, b, d)
+    c.grow([d, a])          # d writes a copy of the shared last page
+    same(a, b, d)
+    c.free(b)
+    same(d, a)
+    c.compact()
+    same(a, d)
+    c.grow([a], 5)
+    same(a, d)
