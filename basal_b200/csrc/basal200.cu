@@ -1324,6 +1324,33 @@ int kv_copy_pages(void* const* pools, const int* layers, const int64_t* page_byt
   return copy_pages_launch<1024>(pools, layers, page_bytes, npools, pages, src, dst, n, st);
 }
 
+// A CTA a key head, whose value heads follow one another, or a cluster of a CTA a value head. Measured for 1 to 256 rows and
+// 2 to 12 value heads a key head (us, h = value heads of the call / SMs): one after another 2.5 + 2.2 rep while the key
+// heads leave SMs idle, and less than any split once they do not; split 4 + 2.2 max(1, h), about 1 more near h = 1 where
+// two CTAs share an SM. So split while h + 1 < rep (20 rows of 2 key heads by 4: 11.1 -> 8.4; by 8: 20.3 -> 14.3).
+template <typename T>
+int gdn_step_launch(const gdnstep::Params& p, int dev, cudaStream_t st) {
+  const int rep = p.Hv / p.Hk;
+  if ((int64_t)p.rows * p.Hv >= (int64_t)g_dev[dev].sms * (rep - 1))
+    return launch_pdl(gdnstep::gdn_step_kernel<T, false>, dim3(p.Hk, p.rows), gdnstep::NT, 0, st, p, 1);
+  const int cluster = rep < 8 ? rep : 8;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(p.Hk * cluster, p.rows);
+  cfg.blockDim = gdnstep::NT;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, gdnstep::gdn_step_kernel<T, true>, p, cluster) != cudaSuccess) return launched();
+  return launched();
+}
+
 int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   if (p.rows < 0 || p.Hk <= 0 || p.Hv <= 0 || p.slots < 0) return BASAL200_ERR_ARG;
   if (p.Hv % p.Hk) return BASAL200_ERR_SHAPE;
@@ -1341,9 +1368,7 @@ int gdn_step(const gdnstep::Params& p, int dt, cudaStream_t st) {
   int dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  const dim3 grid(p.Hk, p.rows);
-  if (dt == BASAL200_BF16) return launch_pdl(gdnstep::gdn_step_kernel<__nv_bfloat16>, grid, gdnstep::NT, 0, st, p);
-  return launch_pdl(gdnstep::gdn_step_kernel<__half>, grid, gdnstep::NT, 0, st, p);
+  return dt == BASAL200_BF16 ? gdn_step_launch<__nv_bfloat16>(p, dev, st) : gdn_step_launch<__half>(p, dev, st);
 }
 
 // A row in equal slices: of up to 32768 tokens (the history is read once a slice), smaller where few rows would leave

@@ -6,10 +6,12 @@
 // is read once into registers (all of a thread's loads are issued before the input steps, which run while they arrive,
 // and the next head's before the current one's output is summed), updated there and written once. A CTA of 256 threads
 // takes a row's key head and its value heads one after another (they share k and q, and the CTA alone reads and writes
-// their convolution inputs); two CTAs an SM keep 128 KB of state in flight. 256 rows of 32 heads: 174 us, 1.10 GB at
-// 6.3 TB/s (96% of a copy's rate); one row 6.8 us, its latency. Splitting a head's columns over a cluster of 8 CTAs for
-// few rows gained 0.2 us at one row and lost from 4 rows on (16 rows: 29 us against 10.9); a cluster of a CTA for each
-// value head gained 0.6 us up to 4 rows and lost from 8 on (256 rows: 237 us, no next head to load ahead).
+// their convolution inputs); two CTAs an SM keep 128 KB of state in flight. 256 rows of 32 heads: 175 us, 1.10 GB at
+// 6.3 TB/s (96% of a copy's rate). Where few rows leave SMs idle, each value head gets a CTA of
+// its own: those of a key head form a cluster (of up to 8, which then take every 8th head), each computes k and q for
+// itself, and the first writes the key head's new inputs after a barrier of the cluster that the others only arrive at:
+// one row of 16 key heads by 2 6.1 us against 6.8, 10 rows of 2 by 8 8.4 against 20.3 (the rule is at the launch).
+// Splitting a head's columns over a cluster as well gained 0.2 us at one row.
 #pragma once
 #include "hybrid.cuh"
 
@@ -85,40 +87,45 @@ constexpr int AHEAD = 6;  // value heads whose inputs are prepared at a time
 constexpr int NT = 256, LANES = 32, BANDS = 8, ROWS = 16;  // 32 lanes of 4 columns by 8 bands of 16 rows of S
 constexpr int GROUPS = ROWS / 4;
 
-// grid (Hk, rows). A column's sums over the rows of S are a binary tree over groups of 4 rows.
-template <typename T>
-__global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p) {
+// grid (Hk * cluster, rows); SPLIT: clusters of `cluster` along x, else cluster is 1. A column's sums over the rows of S are
+// a binary tree over groups of 4 rows.
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p, int cluster_arg) {
   __shared__ __align__(16) float sq[128], sk[128], sv[AHEAD][128];
   __shared__ float sbeta[AHEAD], sdecay[AHEAD];
   __shared__ __align__(16) float4 part[2][BANDS][LANES];
   pdl_wait();
   pdl_launch();
-  const int h = blockIdx.x, b = blockIdx.y, rep = p.Hv / p.Hk;
+  const int cluster = SPLIT ? cluster_arg : 1;
+  const int h = blockIdx.x / cluster, rank = blockIdx.x % cluster, b = blockIdx.y, rep = p.Hv / p.Hk;
+  const int heads = (rep - rank + cluster - 1) / cluster;  // of this CTA: rank, rank + cluster, ..
+  const int head0 = h * rep + rank;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int band = threadIdx.x / LANES, mine = threadIdx.x % LANES, col = mine * 4;
   const int C = (2 * p.Hk + p.Hv) * 128;
-  T* out = static_cast<T*>(p.o) + ((int64_t)b * p.Hv + h * rep) * 128;
+  T* out = static_cast<T*>(p.o) + ((int64_t)b * p.Hv + head0) * 128;
   int64_t slot;
   const int ok = row_slot(p, b, &slot);
-  if (ok <= 0) {
-    if (ok < 0 && threadIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadSlot);
-    for (int i = threadIdx.x; i < rep * 128; i += NT) out[i] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
+  if (ok <= 0) {  // the same in every CTA of a cluster
+    if (ok < 0 && rank == 0 && threadIdx.x == 0) atomicOr(&g_fault, (unsigned)kFaultBadSlot);
+    for (int i = threadIdx.x; i < heads * 128; i += NT)
+      out[i / 128 * cluster * 128 + i % 128] = hybrid::from_f<T>(ok < 0 ? NAN : 0.0f);
     return;
   }
   const T* x = static_cast<const T*>(p.proj) + b * p.ld;
   T* tail = static_cast<T*>(p.tail) + slot * 3 * C;
   const T* conv = static_cast<const T*>(p.conv);
-  float4* S = reinterpret_cast<float4*>(p.state + ((slot * p.Hv + h * rep) * 128 + band * ROWS) * 128 + col);
+  float4* S = reinterpret_cast<float4*>(p.state + ((slot * p.Hv + head0) * 128 + band * ROWS) * 128 + col);
   float4 s[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
 
-  for (int r = 0; r < rep; ++r) {
+  for (int r = 0; r < heads; ++r) {
     if (r % AHEAD == 0) {  // q and k (once) and the next heads' v, beta and decay: a warp each, 4 channels a lane
-      const int heads = min(AHEAD, rep - r);
-      for (int t = warp + (r ? 2 : 0); t < 2 + heads; t += NT / 32) {
+      const int next = min(AHEAD, heads - r);
+      for (int t = warp + (r ? 2 : 0); t < 2 + next; t += NT / 32) {
         float y[4];
-        const int vh = h * rep + r + t - 2;
+        const int vh = head0 + (r + t - 2) * cluster;
         conv4(x, tail, conv, C, (t < 2 ? t * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + vh * 128) + lane * 4, y);
         if (t < 2) {
           float ss = 0.0f;
@@ -140,6 +147,8 @@ __global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p) {
         }
       }
       __syncthreads();
+      // this CTA has read the key head's convolution inputs
+      if (SPLIT && r == 0) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
     const float4 v = *reinterpret_cast<const float4*>(&sv[r % AHEAD][col]);
     const float beta = sbeta[r % AHEAD], decay = sdecay[r % AHEAD];
@@ -174,8 +183,8 @@ __global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p) {
         sum[a] = fma4(qq[i], e, sum[a]);
       }
     }
-    if (r + 1 < rep) {  // the next head's state
-      S += 128 * 32;
+    if (r + 1 < heads) {  // the next head's state
+      S += cluster * 128 * 32;
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) s[i] = S[i * 32];
     }
@@ -184,14 +193,16 @@ __global__ void __launch_bounds__(NT, 2) gdn_step_kernel(const Params p) {
     if (band == 0) {
       const float4 o = tree<BANDS>(&part[1][0][mine], LANES);
       T y[4] = {hybrid::from_f<T>(o.x), hybrid::from_f<T>(o.y), hybrid::from_f<T>(o.z), hybrid::from_f<T>(o.w)};
-      *reinterpret_cast<uint2*>(out + r * 128 + col) = *reinterpret_cast<const uint2*>(y);
+      *reinterpret_cast<uint2*>(out + r * cluster * 128 + col) = *reinterpret_cast<const uint2*>(y);
     }
   }
 
-  // the convolution's last inputs (the loop's barriers came after every read of them)
-  for (int i = threadIdx.x; i < (2 + rep) * LANES; i += NT) {
+  // the convolution's last inputs: of this CTA's value heads (the loop's barriers came after every read of them), and the
+  // key head's by the first CTA once the others have read them
+  if (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  for (int i = threadIdx.x + (rank == 0 ? 0 : 2 * LANES); i < (2 + heads) * LANES; i += NT) {
     const int which = i / LANES;
-    const int c = (which < 2 ? which * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + (h * rep + which - 2) * 128) +
+    const int c = (which < 2 ? which * p.Hk * 128 + h * 128 : 2 * p.Hk * 128 + (head0 + (which - 2) * cluster) * 128) +
                   i % LANES * 4;
     const uint2 a = *reinterpret_cast<const uint2*>(tail + C + c), d = *reinterpret_cast<const uint2*>(tail + 2 * C + c);
     *reinterpret_cast<uint2*>(tail + c) = a;

@@ -74,7 +74,7 @@ def step(ops, x, slots=None):
 
 @pytest.mark.parametrize("dtype", [BF, FP16])
 @pytest.mark.parametrize("rows, spare, Hk, Hv", [(1, 0, 16, 32), (3, 4, 1, 1), (5, 2, 2, 6), (2, 0, 4, 4), (40, 7, 1, 3),
-                                                 (2, 1, 1, 8)])
+                                                 (2, 1, 1, 8), (3, 0, 1, 12), (140, 3, 1, 12), (4, 2, 3, 30)])
 def test_gdn_step(ops, dtype, rows, spare, Hk, Hv):
     x = inputs(rows, rows + spare, Hk, Hv, dtype, seed=rows)
     order = torch.randperm(rows + spare, generator=torch.Generator().manual_seed(rows)).tolist()[:rows]
