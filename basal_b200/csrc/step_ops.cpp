@@ -67,6 +67,9 @@ T* ptr_or_null(const OptTensor& t) {
   return get(t) ? static_cast<T*>(t->data_ptr()) : nullptr;
 }
 
+// t contiguous, of type s (a to() that changes nothing still costs a trip through the dispatcher)
+Tensor as(const Tensor& t, at::ScalarType s) { return t.scalar_type() == s ? t.contiguous() : t.to(s).contiguous(); }
+
 bool aligned(const Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 
 // A cache's pages, scales and table, checked.
@@ -247,8 +250,7 @@ Tensor gdn_step(const Tensor& proj_in, const Tensor& tail, const Tensor& conv_in
     proj = at::empty({rows, (width + 7) / 8 * 8}, proj_in.options()).narrow(1, 0, width);
     proj.copy_(proj_in);
   }
-  const Tensor conv = conv_in.to(dt).contiguous(), A_log = A_log_in.to(at::kFloat).contiguous(),
-               dt_bias = dt_bias_in.to(dt).contiguous();
+  const Tensor conv = as(conv_in, dt), A_log = as(A_log_in, at::kFloat), dt_bias = as(dt_bias_in, dt);
   Tensor o = at::empty({rows, Hv, 1, 128}, proj_in.options());
   done(what, basal200_gdn_step(ptr(proj), code(proj), rows > 1 ? proj.stride(0) : (width + 3) / 4 * 4, ptr(tail), ptr(conv),
                                static_cast<const float*>(ptr(A_log)), ptr(dt_bias), (int)b_off, (int)a_off,
