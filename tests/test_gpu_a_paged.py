@@ -361,6 +361,19 @@ def test_append_8bit_equals_the_activation_quantiser(ops):
     assert torch.equal(pool.scales[0][at].transpose(1, 2).reshape(-1), s.view(-1))
 
 
+@pytest.mark.parametrize("dtype, size", [(FP16, 2e-7), (FP16, 60000.0), (BF, 1e-39), (BF, 1e38), (BF, 1e-13)])
+def test_append_8bit_of_tiny_and_huge_tokens(ops, dtype, size):
+    """Tokens of the type's smallest and largest values (subnormal ones among them) take the quantiser's codes and scales."""
+    pool = Pool([64], 2, 128, 16, dtype, True, seed=27)
+    x = torch.randn(1, 64, 2, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(28)).clamp(-1, 1)
+    x = (x.double() * size).to(dtype)
+    ops.kv_append(x, x, *pool.full, pool.table, torch.zeros(1, dtype=torch.int32, device="cuda"), None, *pool.scales)
+    q, s = ops.fp8_act_quant(x.view(-1, 128))
+    at = pool.table[0].long()
+    assert torch.equal(pool.full[0].view(torch.uint8)[at].transpose(1, 2).reshape(-1, 128), q.view(torch.uint8))
+    assert torch.equal(pool.scales[1][at].transpose(1, 2).reshape(-1), s.view(-1))
+
+
 def test_append_strided_sources_without_count(ops):
     """[rows, heads, tokens, D] seen as [rows, tokens, heads, D], a slice of a wider projection, and unaligned ones."""
     for fp8 in (False, True):
