@@ -71,6 +71,12 @@ __host__ __device__ __forceinline__ int most_parts(int64_t nt, int least, int ca
   return n < 1 ? 1 : n < cap ? (int)n : cap;
 }
 
+// The query head that lane row r of an item's g-th eight heads reads: its own, or the item's first head, which is always
+// there, where the item has no such head (the lane then drops what it read). An item has 1 to 8 NG heads, from head0.
+__host__ __device__ constexpr int query_head(int head0, int heads, int g, int r) {
+  return head0 + (g * 8 + r < heads ? g * 8 + r : 0);
+}
+
 struct Workspace {
   float* o;  // [rows, H, parts, D] sums of p v, relative to m
   float* m;  // [rows, H, parts] maximum, base 2; NaN: the row is refused
@@ -303,10 +309,10 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
   const int G = p.H / p.Hk;
   const int units = p.Hk * groups;
 
-  // A lane's share of the query of 8 heads from head0: head r's (or zeros past the item's heads).
-  auto load_q = [&](int row, int head0, int live, uint32_t (&w)[QW]) {
-    const bool in = r < live;
-    const TQ* src = static_cast<const TQ*>(p.q) + row * p.q_row + (head0 + (in ? r : 0)) * p.q_head;
+  // A lane's share of the query of an item's g-th eight heads: head g * 8 + r's, or zeros past the item's heads.
+  auto load_q = [&](int row, int head0, int heads, int g, uint32_t (&w)[QW]) {
+    const bool in = g * 8 + r < heads;
+    const TQ* src = static_cast<const TQ*>(p.q) + row * p.q_row + query_head(head0, heads, g, r) * p.q_head;
     if constexpr (!FP8) {
 #pragma unroll
       for (int j = 0; j < QW; ++j) {  // step j / 2: dimensions 8 j + 2c, 8 j + 2c + 1
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
       if (q_for < done) {  // the query loaded early has been taken
         int heads;
         const int h0 = head0_of(unit, &heads);
-        load_q(it_row, h0, heads, qn);
+        load_q(it_row, h0, heads, 0, qn);
         q_for = begun;
       }
     }
@@ -526,7 +532,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
           for (int i = 0; i < QW; ++i) w[i] = qn[i];
         }
       }
-      if (!have) load_q(row, head0 + g * 8, heads - g * 8, w);
+      if (!have) load_q(row, head0, heads, g, w);
       float f = p.scale * 1.4426950408889634f;
       if constexpr (!FP8) {
 #pragma unroll
