@@ -4,7 +4,8 @@ there token by token (hybrid.HybridClassifier.open / step / answer) keeps its ke
 
   PagedKVCache(layers, pages, kv_heads, head_dim, page_size, dtype, fp8, device)
       .add()                  a new, empty sequence -> its number
-      .fork(seq)              a new sequence with seq's tokens, its pages shared and counted (nothing is copied)
+      .fork(seq)              a new sequence with seq's tokens, its pages shared and counted (nothing is copied). What
+                              seq last grew by is appended before: a batch made after the fork brings nothing of it
       .grow(seqs, n)          room for n more tokens in each of seqs: new pages, and a copy of a shared page before it
                               is written (one basal::kv_copy_pages over every layer); raises MemoryError, with nothing
                               changed, when the free pages do not suffice
@@ -31,7 +32,8 @@ E4M3 = torch.float8_e4m3fn
 @dataclasses.dataclass
 class Batch:
     """Some sequences, in order, as the kernels see them: table [rows, width], the lengths [rows] with the tokens that
-    the last grow() made room for, and where those begin."""
+    the last grow() made room for, where those begin and how many they are (0 for a sequence that it did not name, or
+    that was forked since: an append leaves it as it is)."""
     seqs: list
     table: torch.Tensor
     lengths: torch.Tensor
@@ -61,7 +63,7 @@ class PagedKVCache:
         self._row = {}               # the same as an array, made again after a change: a long cache's table is not built
                                      # page by page at every step
         self._length = {}
-        self._new = {}               # tokens that the last grow() made room for
+        self._new = {}               # sequence -> tokens that the last grow() made room for, where it named the sequence
         self._next = 0
 
     @property
@@ -86,7 +88,7 @@ class PagedKVCache:
 
     def add(self):
         seq, self._next = self._next, self._next + 1
-        self._of[seq], self._length[seq], self._new[seq] = [], 0, 0
+        self._of[seq], self._length[seq] = [], 0
         return seq
 
     def fork(self, seq):
@@ -95,6 +97,7 @@ class PagedKVCache:
         self._of[new], self._length[new] = list(pages), self._length[seq]
         for p in pages:
             self._shares[p] += 1
+        self._new.pop(seq, None)  # its last page is shared now
         return new
 
     def free(self, seq):
@@ -102,7 +105,8 @@ class PagedKVCache:
             self._shares[p] -= 1
             if not self._shares[p]:
                 self._free.append(p)
-        del self._of[seq], self._length[seq], self._new[seq]
+        del self._of[seq], self._length[seq]
+        self._new.pop(seq, None)
         self._row.pop(seq, None)
 
     def grow(self, seqs, n=1):
@@ -137,6 +141,7 @@ class PagedKVCache:
             dst.append(new)
         if src:
             ops.kv_copy_pages(self.pools, src, dst)
+        self._new = dict(zip(seqs, n))
         for s, m in zip(seqs, n):
             pages = self._of[s]
             while len(pages) * self.page_size < self._length[s] + m:
@@ -144,7 +149,6 @@ class PagedKVCache:
                 pages.append(self._free.pop())
                 self._shares[pages[-1]] = 1
             self._length[s] += m
-            self._new[s] = m
 
     def batch(self, seqs):
         seqs = list(seqs)
@@ -157,7 +161,8 @@ class PagedKVCache:
                 pages = self._row[s] = np.asarray(self._of[s], np.int32)
             rows[i, :len(pages)] = pages
             rows[i, len(pages):width] = -1
-            rows[i, width:] = self._length[s], self._length[s] - self._new[s], self._new[s]
+            new = self._new.get(s, 0)
+            rows[i, width:] = self._length[s], self._length[s] - new, new
         t = host.to(self.device, non_blocking=True)
         lengths, start, count = t[:, width:].t().contiguous()
         return Batch(seqs, t[:, :width], lengths, start, count)

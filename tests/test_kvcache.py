@@ -160,3 +160,27 @@ def test_batches_follow_every_change(moved):
     same(a, d)
     c.grow([a], 5)
     same(a, d)
+
+
+def test_a_batch_brings_only_what_the_last_grow_made_room_for(moved):
+    """A grown, an ungrown and a forked sequence in one batch: an append with it writes the grown one's tokens and no
+    other position, so no shared page and no token that was appended before."""
+    c = cache()
+    a, b = c.add(), c.add()
+    c.grow([a, b], 2)
+    f = c.fork(b)
+    got = c.batch([b, f])               # forked since: its page is shared
+    assert got.count.tolist() == [0, 0] and got.start.tolist() == got.lengths.tolist() == [2, 2]
+    c.grow([a])
+    got = c.batch([a, b, f])
+    assert got.count.tolist() == [1, 0, 0] and got.start.tolist() == [2, 2, 2] and got.lengths.tolist() == [3, 2, 2]
+    c.grow([b, f], [3, 0])
+    got = c.batch([a, b, f])
+    assert got.count.tolist() == [0, 3, 0] and got.start.tolist() == [3, 2, 2] and got.lengths.tolist() == [3, 5, 2]
+    c.compact()                          # pages move, tokens stay to be appended
+    assert c.batch([b]).count.tolist() == [3]
+    c.free(b)
+    with pytest.raises(MemoryError):
+        c.grow([a], 100)
+    assert c.batch([a, f]).count.tolist() == [0, 0]
+    consistent(c)
