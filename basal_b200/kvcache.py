@@ -129,18 +129,18 @@ class PagedKVCache:
             need += max(0, -(-(length + m) // self.page_size) - len(pages))
         if need > len(self._free):
             raise MemoryError(f"PagedKVCache: {need} pages are needed, {len(self._free)} are free")
-        src, dst = [], []
-        for s in copies:
-            at = self._length[s] // self.page_size
-            old, new = self._of[s][at], self._free.pop()
+        # the copies come first: where they are refused, nothing has changed
+        where = [self._length[s] // self.page_size for s in copies]
+        src = [self._of[s][at] for s, at in zip(copies, where)]
+        dst = [self._free[-1 - i] for i in range(len(copies))]
+        if src:
+            ops.kv_copy_pages(self.pools, src, dst)
+        for s, at, old, new in zip(copies, where, src, dst):
+            self._free.pop()
             self._shares[old] -= 1
             self._shares[new] = 1
             self._of[s][at] = new
             self._row.pop(s, None)
-            src.append(old)
-            dst.append(new)
-        if src:
-            ops.kv_copy_pages(self.pools, src, dst)
         self._new = dict(zip(seqs, n))
         for s, m in zip(seqs, n):
             pages = self._of[s]

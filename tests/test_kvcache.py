@@ -184,3 +184,20 @@ def test_a_batch_brings_only_what_the_last_grow_made_room_for(moved):
         c.grow([a], 100)
     assert c.batch([a, f]).count.tolist() == [0, 0]
     consistent(c)
+
+
+def test_a_copy_that_is_refused_changes_nothing(monkeypatch):
+    c = cache()
+    a = c.add()
+    c.grow([a], 6)
+    b = c.fork(a)
+    before = (c.pages_of(a), c.pages_of(b), c.length(b), c.free_pages, c.batch([a, b]).table.tolist())
+
+    def fails(*a):
+        raise RuntimeError("no copy")
+
+    monkeypatch.setattr(kvcache.ops, "kv_copy_pages", fails)
+    with pytest.raises(RuntimeError):
+        c.grow([b], 5)
+    assert before == (c.pages_of(a), c.pages_of(b), c.length(b), c.free_pages, c.batch([a, b]).table.tolist())
+    consistent(c)
