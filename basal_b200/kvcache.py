@@ -16,8 +16,8 @@ there token by token (hybrid.HybridClassifier.open / step / answer) keeps its ke
       .compact()              moves the live pages to the lowest numbers (one kv_copy_pages) -> how many pages are live
 
 The bookkeeping is on the host; the device sees the pages, and tables and lengths as int32 tensors. A Batch says how things
-were when it was made: after grow, free or compact, make another. The copies run on the current stream: use the cache from
-one stream, or order the streams.
+were when it was made: after grow, free or compact, make another (outside of a captured graph). The copies run on the
+current stream: use the cache from one stream, or order the streams.
 """
 import dataclasses
 
@@ -152,6 +152,9 @@ class PagedKVCache:
 
     def batch(self, seqs):
         seqs = list(seqs)
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: a graph would keep the host memory that a batch is copied from: make the "
+                               "batch before the capture, and copy later ones over its tensors")
         width = max([len(self._known(s)) for s in seqs], default=0) or 1
         host = torch.empty((len(seqs), width + 3), dtype=torch.int32, pin_memory=self.device.type == "cuda")
         rows = host.numpy()

@@ -201,3 +201,14 @@ def test_a_copy_that_is_refused_changes_nothing(monkeypatch):
         c.grow([b], 5)
     assert before == (c.pages_of(a), c.pages_of(b), c.length(b), c.free_pages, c.batch([a, b]).table.tolist())
     consistent(c)
+
+
+def test_no_batch_inside_a_captured_graph(moved, monkeypatch):
+    """A graph would replay the copy from host memory that is used for something else by then."""
+    c = cache()
+    a = c.add()
+    c.grow([a], 2)
+    c.device = torch.device("cuda")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        c.batch([a])
