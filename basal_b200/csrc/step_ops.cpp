@@ -72,6 +72,10 @@ Tensor as(const Tensor& t, at::ScalarType s) { return t.scalar_type() == s ? t.c
 
 bool aligned(const Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 
+// A copy of t in memory of its own, contiguous and aligned (contiguous() hands back a view that is contiguous where it
+// lies: at an odd offset, or one row with any row stride).
+Tensor copied(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+
 // A cache's pages, scales and table, checked.
 struct Cache {
   int64_t pages, page, head, token, s_page = 0, s_head = 0, table_row;
@@ -132,7 +136,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, con
                     " heads of ", c.D);
   need_int32("lengths", lengths_in, {rows});
   const bool fits = q_in.stride(2) == 1 && q_in.stride(0) % 8 == 0 && q_in.stride(1) % 8 == 0 && aligned(q_in, 16);
-  const Tensor q = fits ? q_in : q_in.contiguous(), lengths = lengths_in.contiguous();
+  const Tensor q = fits ? q_in : copied(q_in), lengths = lengths_in.contiguous();
   const c10::cuda::CUDAGuard guard(dev);
   Tensor out = at::empty({rows, H, D}, q.options());
   const int r = to_int(what, rows), h = to_int(what, H), w = to_int(what, window);
@@ -167,7 +171,7 @@ void kv_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, co
     count = count_in->contiguous();
   }
   auto fit = [](const Tensor& x) {
-    return x.stride(3) == 1 && (x.stride(0) | x.stride(1) | x.stride(2)) % 8 == 0 && aligned(x, 16) ? x : x.contiguous();
+    return x.stride(3) == 1 && (x.stride(0) | x.stride(1) | x.stride(2)) % 8 == 0 && aligned(x, 16) ? x : copied(x);
   };
   const Tensor k = fit(k_in), v = fit(v_in), start = start_in.contiguous();
   const c10::cuda::CUDAGuard guard(dev);
@@ -250,7 +254,9 @@ Tensor gdn_step(const Tensor& proj_in, const Tensor& tail, const Tensor& conv_in
     proj = at::empty({rows, (width + 7) / 8 * 8}, proj_in.options()).narrow(1, 0, width);
     proj.copy_(proj_in);
   }
-  const Tensor conv = as(conv_in, dt), A_log = as(A_log_in, at::kFloat), dt_bias = as(dt_bias_in, dt);
+  Tensor conv = as(conv_in, dt);
+  if (!aligned(conv, 16)) conv = copied(conv);
+  const Tensor A_log = as(A_log_in, at::kFloat), dt_bias = as(dt_bias_in, dt);
   Tensor o = at::empty({rows, Hv, 1, 128}, proj_in.options());
   done(what, basal200_gdn_step(ptr(proj), code(proj), rows > 1 ? proj.stride(0) : (width + 3) / 4 * 4, ptr(tail), ptr(conv),
                                static_cast<const float*>(ptr(A_log)), ptr(dt_bias), (int)b_off, (int)a_off,

@@ -461,3 +461,23 @@ def test_copy_and_append_captured(ops):
     p[0, 0] = -1
     g.replay()
     assert torch.equal(p[0, 4], p[0, 0]) and torch.equal(p[0, 5], p[0, 1]) and int(p[0, 3, 0]) == 48
+
+
+# --- inputs that are contiguous and not aligned --------------------------------------------------------------------
+@pytest.mark.parametrize("offset", [1, 3, 4, 8])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_one_row_at_any_offset(ops, fp8, offset):
+    """One row's query, key and value as slices of a projection at any column: contiguous views, most not 16-byte
+    aligned, one with a row stride that is no multiple of 8."""
+    pool, same = (Pool([70], 2, 128, 16, BF, fp8, seed=29) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(30)
+    proj = torch.randn(1, offset + 8 * 128 + 3, device="cuda", generator=g).to(BF)
+    q = proj[:, offset:offset + 512].view(1, 4, 128)
+    k, v = (proj[:, offset + at:offset + at + 256].view(1, 1, 2, 128) for at in (512, 768))
+    assert q.is_contiguous() and k.is_contiguous()
+    start = torch.tensor([69], dtype=torch.int32, device="cuda")
+    ops.kv_append(k, v, *pool.full, pool.table, start, None, *pool.scales)
+    ops.kv_append(k.clone(), v.clone(), *same.full, same.table, start, None, *same.scales)
+    for a, b in zip(pool.full, same.full):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(attend(ops, pool, q, 0.09), attend(ops, same, q.clone(), 0.09))

@@ -529,3 +529,18 @@ def test_outputs_do_not_need_gradients(ops):
     with torch.no_grad():
         b = ops.paged_attention(x["q"].requires_grad_(), x["k"], x["v"], x["table"], x["lengths"], 0.125)
     assert torch.equal(a, b) and not b.requires_grad
+
+
+# --- inputs that are contiguous and not aligned --------------------------------------------------------------------
+@pytest.mark.parametrize("offset", [1, 4])
+def test_gdn_step_inputs_at_any_offset(ops, offset):
+    """One row's projection and the convolution's weights as contiguous views that are not aligned."""
+    a, b = (inputs(1, 1, 2, 4, BF, seed=31) for _ in range(2))
+    for name in ("proj", "conv"):
+        x = b[name]
+        flat = torch.zeros(x.numel() + offset, dtype=BF, device="cuda")
+        flat[offset:] = x.reshape(-1)
+        b[name] = flat[offset:].view(x.shape)
+        assert b[name].is_contiguous()
+    assert torch.equal(step(ops, b), step(ops, a))
+    assert torch.equal(a["state"], b["state"]) and torch.equal(a["tail"], b["tail"])
