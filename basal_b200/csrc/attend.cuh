@@ -12,7 +12,7 @@
 // current ones, and no warp waits for another but where they join an item's result. An item that is a whole row is
 // written at once; parts of longer rows go to the workspace and attend_join_kernel adds them up. Measured: 64 rows of up
 // to 8192 (16 heads over 4 of 128, 543 MB) 94 us, 89% of a copy's rate, waiting for memory; 8-bit pages, 128 rows of up to
-// 4001 (32 over 8, 541 MB) 107 us at 2 instructions a cycle an SM; one row of 200 6.5 us, of which the instructions'
+// 4001 (32 over 8, 541 MB) 113 us at 2 instructions a cycle an SM; one row of 200 6.5 us, of which the instructions'
 // first fetches are the larger part.
 //
 // Arithmetic, per 16 tokens: S^T [16 tokens x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T on mma.sync m16n8k16 with
@@ -24,8 +24,10 @@
 // Weights are 2^(z - ref) with z the logit times log2 e and ref a maximum that is raised only when some z passes it by
 // more than 8: a tile then costs one vote instead of a maximum across lanes and a rescaling of the sums, and weights
 // stay below 2^8, which changes no relative error (sums and outputs are fp32). An 8-bit key's scale multiplies its
-// logit, a value's scale its weight, relative to a power of two that follows the largest scale seen; the query is
-// brought to fp16 by a power of two of its own; so neither can leave fp16's range.
+// logit, a value's scale its weight; the query and those products are brought to fp16 by powers of two of their own, the
+// head's largest query value and the largest product of a weight and a scale that it has seen (over_top), so that neither
+// the largest nor what counts beside it leaves fp16's range: a product is off by its rounding (2^-11, 2^-22 split in two) or,
+// below 2^-18 of the largest, by 2^-29 of the largest.
 #pragma once
 #include "paged.cuh"
 
@@ -203,6 +205,18 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // The reference before any logit: finite, so that a difference with it is never NaN.
 constexpr float NO_MAX = -3.0e38f;
 constexpr float SLACK = 8.0f;
+
+// 8-bit values: a head's weights times their scales are handed to the MMA over a power of two near the largest such
+// product that the head has seen, `top`: 2^4 to 2^5 is the largest one's size (below 2^15 for a scale of up to 4 times
+// top under a weight of 2^8, what is taken before top is raised). Only the product counts: a far larger scale under a weight
+// that is next to nothing leaves the others what they are. top is kept from 2^-122 on, so that both powers exist.
+constexpr float TOP_LEAST = 1.8807909613156600e-37f;  // 2^-122
+__device__ __forceinline__ float over_top(float top) {  // 2^4 / 2^floor(log2 top)
+  return __uint_as_float((258u << 23) - (__float_as_uint(top) & 0x7F800000u));
+}
+__device__ __forceinline__ float times_top(float top) {  // its inverse
+  return __uint_as_float((__float_as_uint(top) & 0x7F800000u) - (4u << 23));
+}
 
 template <bool FP8, int D, int NG>
 struct AttendShape {
@@ -501,7 +515,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
   // ---- the computing side ----
   uint32_t q[NG][QW];
   float o[NG][MT][4], mx[NG][2], sum[NG][2], fac[NG][2];  // mx: the weights' reference, base 2
-  float ref_v;                                            // 8-bit: the power of two that the values' scales are over
+  float top_p[NG][2];                                     // 8-bit: the largest product of a weight and its value's scale
   int joined = 0;                                         // joins so far, the same in every warp
   bool alive = true;                                      // no wait has given up
 
@@ -520,7 +534,6 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
     int heads;
     const int head0 = head0_of(unit, &heads);
 
-    ref_v = 0.0f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint32_t w[QW];
@@ -561,6 +574,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
         fac[g][1] = __shfl_sync(0xffffffffu, f, c * 8 + 4);  // head 2c + 1
       }
       mx[g][0] = mx[g][1] = NO_MAX;
+      top_p[g][0] = top_p[g][1] = TOP_LEAST;
       sum[g][0] = sum[g][1] = 0.0f;
 #pragma unroll
       for (int t = 0; t < MT; ++t) o[g][t][0] = o[g][t][1] = o[g][t][2] = o[g][t][3] = 0.0f;
@@ -621,7 +635,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
       }
       const bool edge = at < first || at + TT > n;
       float z[SUB][NG][4], hi[NG][2];
-      bool up = FP8 && top_v > ref_v;
+      bool up = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
 #pragma unroll
@@ -643,20 +657,10 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
         for (int h = 0; h < 2; ++h) {
           hi[g][h] = fmaxf(z[0][g][h], z[0][g][h + 2]);
           if (SUB == 2) hi[g][h] = fmaxf(hi[g][h], fmaxf(z[SUB - 1][g][h], z[SUB - 1][g][h + 2]));
-          up |= hi[g][h] > mx[g][h] + SLACK;
+          up |= hi[g][h] > mx[g][h] + SLACK || (FP8 && top_v > 4.0f * top_p[g][h]);
         }
       }
       if (__any_sync(0xffffffffu, up)) {  // raise the references to what has been seen, and the sums with them
-        float grow = 1.0f;
-        if (FP8) {
-#pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, x));
-          if (top_v > ref_v) {
-            const uint32_t e = min((__float_as_uint(top_v) >> 23) + 2u, 253u);
-            grow = ref_v * __uint_as_float((254u - e) << 23);
-            ref_v = __uint_as_float(e << 23);
-          }
-        }
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -668,21 +672,24 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
             float f = ex2(mx[g][h] - m);
             mx[g][h] = m;
             sum[g][h] *= f;
-            f *= grow;
+            if (FP8) {
+              float t = 0.0f;
+#pragma unroll
+              for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) t = fmaxf(t, ex2(z[u][g][h + 2 * i] - m) * fabsf(sv[u][i]));
+#pragma unroll
+              for (int x = 4; x <= 16; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+              t = fmaxf(fmaxf(top_p[g][h] * f, t), TOP_LEAST);
+              f = f * times_top(top_p[g][h]) * over_top(t);
+              top_p[g][h] = t;
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               o[g][i][h] *= f;
               o[g][i][h + 2] *= f;
             }
           }
-      }
-      if (FP8) {
-        const float inv = ref_v > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(ref_v)) : 0.0f;
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-          sv[u][0] *= inv;
-          sv[u][1] *= inv;
-        }
       }
       uint32_t ph[SUB][NG][2], pl[SUB][NG][2];
 #pragma unroll
@@ -696,7 +703,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
           sum[g][1] += w[1] + w[3];
           if (FP8) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] *= sv[u][i >> 1];
+            for (int i = 0; i < 4; ++i) w[i] = w[i] * sv[u][i >> 1] * over_top(top_p[g][i & 1]);
           }
           const uint32_t h0 = MM::pack(w[0], w[1]), h1 = MM::pack(w[2], w[3]);
           ph[u][g][0] = transposed(h0);
@@ -785,9 +792,9 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
         alive = warp_wait(&js->read, joined, js);  // the last join has been read
         if (!alive) break;
         if (JHEADS == 8 || c >> 1 == half) {
-          const float back = FP8 ? ref_v : 1.0f;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const float back = FP8 ? times_top(top_p[g][h]) : 1.0f;
             const int head = 2 * (c & (JHEADS / 2 - 1)) + h;
             if (r == 0) {
               join_m[warp * JHEADS + head] = parts < 0 ? NAN : mx[g][h];

@@ -481,3 +481,36 @@ def test_one_row_at_any_offset(ops, fp8, offset):
     for a, b in zip(pool.full, same.full):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     assert torch.equal(attend(ops, pool, q, 0.09), attend(ops, same, q.clone(), 0.09))
+
+
+# --- 8-bit values under weights of any size ------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, FP16])
+@pytest.mark.parametrize("n", [300, 6000])
+@pytest.mark.parametrize("ratio", [16, 20, 24, 40, 80, 100])
+def test_attention_8bit_large_scale_of_an_unlikely_token(ops, dtype, n, ratio):
+    """A token whose value scale is 2^ratio times the others' and whose logit is 60 below theirs (a weight of 2^-86): what
+    counts is the product of scale and weight, from nothing (2^16) to nearly all (2^100) of the output."""
+    pool = Pool([n, 40], 2, 128, 16, dtype, True, seed=32)
+    g = torch.Generator(device="cuda").manual_seed(33)
+    one = torch.randn(2, 2, 1, 128, device="cuda", generator=g).expand(2, 2, 2, 128) * 2  # a key head's queries alike
+    q = (one * torch.tensor([1.0, 0.9], device="cuda")[:, None]).reshape(2, 4, 128).to(dtype)
+    for r, at in ((0, n // 2 + 3), (0, 5), (1, 17)):
+        page, off = pool.table[r, at // 16].long(), at % 16
+        x = one[r, :, 0]
+        codes, s = quantised(x * (-60 / (128 ** -0.5 * x.square().sum(-1, keepdim=True))))
+        pool.full[0].view(torch.uint8)[page, :, off] = codes.view(torch.uint8)
+        pool.scales[0][page, :, off] = s
+        pool.scales[1][page, :, off] *= 2.0 ** ratio
+    got = attend(ops, pool, q, 128 ** -0.5)
+    if dtype == BF or ratio < 100:
+        return check(ops, pool, q, 128 ** -0.5, got)
+    # 2^100 e^-60 is 2^13.4 (2^22 for the queries of 0.9), and values reach 4: past fp16's largest value, 65504, whose rounding
+    # is an infinity; the others are compared to 2^-6, well above check()'s bound for them
+    for r in range(2):
+        k, v = pool.row(r)
+        p = torch.softmax(q[r].double().view(2, 2, 128) @ k.transpose(1, 2) * 128 ** -0.5, -1)
+        o, a = (p @ v).view(4, 128), (p @ v.abs()).view(4, 128)
+        y = got[r].double()
+        large, small = o.abs() > 65520 + 2.0 ** -6 * a, o.abs() < 65504 - 2.0 ** -6 * a
+        assert (y[large] == o[large].sign() * float("inf")).all()
+        assert ((y - o).abs() <= 2.0 ** -6 * a)[small].all()
