@@ -514,3 +514,29 @@ def test_attention_8bit_large_scale_of_an_unlikely_token(ops, dtype, n, ratio):
         large, small = o.abs() > 65520 + 2.0 ** -6 * a, o.abs() < 65504 - 2.0 ** -6 * a
         assert (y[large] == o[large].sign() * float("inf")).all()
         assert ((y - o).abs() <= 2.0 ** -6 * a)[small].all()
+
+
+@pytest.mark.parametrize("dtype, fp8", [(BF, False), (FP16, False), (BF, True), (FP16, True)])
+@pytest.mark.parametrize("bits", [20, 24, 26])
+@pytest.mark.parametrize("n, first", [(300, 0), (300, 170), (5000, 2)])
+def test_attention_of_small_weights_beside_a_token_without_a_value(ops, dtype, fp8, bits, n, first):
+    """A token that takes nearly all of the weight and whose value is zero: the output is made of weights of 2^-bits, which
+    count as they are, not to the largest one's rounding (all logits but one are equal, so that errors would not cancel)."""
+    pool = Pool([n, 40], 1, 128, 16, dtype, fp8, seed=34)
+    g = torch.Generator(device="cuda").manual_seed(35)
+    q = torch.randn(1, 1, 128, device="cuda", generator=g).expand(2, 4, 128).to(dtype)
+    scale = 128 ** -0.5
+    for r, at in ((0, first), (1, 3)):
+        x = q[r, 0].double() * (bits * 0.6931471805599453 / (scale * q[r, 0].double().square().sum()))
+        size = int(pool.lengths[r])
+        pages, off = pool.table[r].long()[torch.arange(size, device="cuda") // 16], torch.arange(size, device="cuda") % 16
+        sink = torch.zeros(size, 1, 1, device="cuda")
+        sink[at] = 1
+        for i, y in enumerate((sink * x.float(), torch.randn(size, 1, 128, device="cuda", generator=g).abs() * 1000 * (1 - sink))):
+            if fp8:
+                codes, s = quantised(y)
+                pool.full[i].view(torch.uint8)[pages, :, off] = codes.view(torch.uint8)
+                pool.scales[i][pages, :, off] = s
+            else:
+                pool.full[i][pages, :, off] = y.to(dtype)
+    check(ops, pool, q, scale, attend(ops, pool, q, scale))
