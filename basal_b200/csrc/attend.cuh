@@ -24,7 +24,7 @@
 // fp16 while p is within 2^-16 of the largest).
 // Weights are 2^(z - ref) with z the logit times log2 e and ref a maximum that is raised only when some z passes it by
 // more than 8 (2 for fp16 pages): a tile then costs one vote instead of a maximum across lanes and a rescaling of the sums,
-// and weights stay below 2^8 (2^15), which changes no relative error (sums and outputs are fp32). An 8-bit key's scale multiplies its
+// and the largest weight is 2^-8 to 1 (2^13 to 2^15), which changes no relative error (sums and outputs are fp32). An 8-bit key's scale multiplies its
 // logit, a value's scale its weight; the query and those products are brought to fp16 by powers of two of their own, the
 // head's largest query value and the largest product of a weight and a scale that it has seen (over_top), so that neither
 // the largest nor what counts beside it leaves fp16's range: a product is off by its rounding (2^-11, 2^-22 split in two) or,
@@ -206,8 +206,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // The reference before any logit: finite, so that a difference with it is never NaN.
 constexpr float NO_MAX = -3.0e38f;
 // 8-bit values: a head's weights times their scales are handed to the MMA over a power of two near the largest such
-// product that the head has seen, `top`: 2^4 to 2^5 is the largest one's size (below 2^15 for a scale of up to 4 times
-// top under a weight of 2^8, what is taken before top is raised). Only the product counts: a far larger scale under a weight
+// product that the head has seen, `top`: 2^4 to 2^5 is the largest one's size (below 2^15 for a scale of up to 2^10 times
+// top, which is what is taken before top is raised: weights are below 1, the largest one 2^-8 or more). Only the product counts: a far larger scale under a weight
 // that is next to nothing leaves the others what they are. top is kept from 2^-122 on, so that both powers exist.
 constexpr float TOP_LEAST = 1.8807909613156600e-37f;  // 2^-122
 __device__ __forceinline__ float over_top(float top) {  // 2^4 / 2^floor(log2 top)
@@ -297,11 +297,12 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
   // one's 2^-11, and by 2^-8 in bf16: those are split in two.
   constexpr bool SPLIT = !(FP8 && std::is_same<TQ, __nv_bfloat16>::value);
   // A head's reference is set LIFT below the largest logit and raised when one passes that by SLACK: weights reach
-  // 2^(LIFT + SLACK), and the largest is at least 2^LIFT. In fp16, whose smallest step is 2^-24, the weights of a long row
-  // lie far below its first token's or another one's that takes nearly all, so the largest is put close to fp16's top: a
-  // weight down to 2^-27 of the largest keeps its 11 bits, a smaller one is held to 2^-38 of it.
+  // 2^(LIFT + SLACK), and the largest is at least 2^LIFT. They stay below 1, so that a sum of them times values near the
+  // type's largest overflows only where the softmax's own terms would. Not so in fp16, whose smallest step is 2^-24 (and
+  // whose values end at 2^16): the weights of a long row lie far below one token's that takes nearly all, so the largest is
+  // put close to fp16's top: a weight down to 2^-27 of the largest keeps its 11 bits, a smaller one is held to 2^-38 of it.
   constexpr bool F16 = !FP8 && std::is_same<TQ, __half>::value;
-  constexpr float LIFT = F16 ? 13.0f : 0.0f, SLACK = F16 ? 2.0f : 8.0f;
+  constexpr float LIFT = F16 ? 13.0f : -8.0f, SLACK = F16 ? 2.0f : 8.0f;
   constexpr int ROWS_STEP = 32 / CH;                 // token rows that one warp-wide load covers
   constexpr int JC = CH / 4 > 0 ? CH / 4 : 1;          // 8-bit: 16-byte chunks of a key that a lane feeds to the MMA
   constexpr int VB = RB / 8 < 16 ? RB / 8 : 16;      // 8-bit: bytes of a value load
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
         for (int h = 0; h < 2; ++h) {
           hi[g][h] = fmaxf(z[0][g][h], z[0][g][h + 2]);
           if (SUB == 2) hi[g][h] = fmaxf(hi[g][h], fmaxf(z[SUB - 1][g][h], z[SUB - 1][g][h + 2]));
-          up |= hi[g][h] > mx[g][h] + (LIFT + SLACK) || (FP8 && top_v > 4.0f * top_p[g][h]);
+          up |= hi[g][h] > mx[g][h] + (LIFT + SLACK) || (FP8 && top_v > 1024.0f * top_p[g][h]);
         }
       }
       if (__any_sync(0xffffffffu, up)) {  // raise the references to what has been seen, and the sums with them

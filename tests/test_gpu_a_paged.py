@@ -540,3 +540,27 @@ def test_attention_of_small_weights_beside_a_token_without_a_value(ops, dtype, f
             else:
                 pool.full[i][pages, :, off] = y.to(dtype)
     check(ops, pool, q, scale, attend(ops, pool, q, scale))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attention_of_values_near_the_largest(ops, fp8):
+    """Values of 1.5e38 under logits that rise by up to 2^7.5 within a row: the output is 1.5e38 too, and no sum on the way
+    there passes 3.4e38."""
+    pool = Pool([200, 40], 1, 128, 16, BF, fp8, seed=36)
+    g = torch.Generator(device="cuda").manual_seed(37)
+    q = torch.randn(1, 1, 128, device="cuda", generator=g).expand(2, 4, 128).to(BF)
+    x = q[0, 0].double() / (128 ** -0.5 * q[0, 0].double().square().sum()) * 0.6931471805599453  # a logit of 1, base 2
+    for r, size in enumerate((200, 40)):
+        pages, off = pool.table[r].long()[torch.arange(size, device="cuda") // 16], torch.arange(size, device="cuda") % 16
+        z = torch.full((size, 1, 1), -40.0, device="cuda")
+        for at, up in ((0, 0.0), (20, 5.0), (64, 7.0), (128, 7.5)):
+            z[at:at + 1] = up
+        values = torch.full((size, 1, 128), 1.5e38, device="cuda") * torch.where(torch.arange(128, device="cuda") % 3 > 0, 1, -1)
+        for i, y in enumerate((z * x.float(), values)):
+            if fp8:
+                codes, s = quantised(y)
+                pool.full[i].view(torch.uint8)[pages, :, off] = codes.view(torch.uint8)
+                pool.scales[i][pages, :, off] = s
+            else:
+                pool.full[i][pages, :, off] = y.to(BF)
+    check(ops, pool, q, 128 ** -0.5, attend(ops, pool, q, 128 ** -0.5))
