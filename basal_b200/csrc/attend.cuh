@@ -251,7 +251,7 @@ struct __align__(16) ItemInfo {
 
 // The joins' state in shared memory, counted over the kernel's life: parts left by the warps, joins read by the warps that
 // join, and whether a wait gave up. Waits are bounded (a caller that changes the lengths while the kernel reads them can
-// make its warps disagree on the items): the kernel then records a fault bit and ends.
+// make its warps disagree on the items): the kernel then records a fault bit, refuses the rows and ends.
 struct JoinState {
   int left, read, gave_up;
 };
@@ -282,6 +282,14 @@ __device__ __forceinline__ bool wait_for(const int* p, int want, JoinState* js) 
 // The same for a warp, whose lanes may have seen different answers: one for all of them.
 __device__ __forceinline__ bool warp_wait(const int* p, int want, JoinState* js) {
   return __all_sync(0xffffffffu, wait_for(p, want, js));
+}
+
+// What a wait that gave up leaves behind: every row refused (NaN pairs `nan` in the output, NaN maxima of the parts), since
+// it is not known which items its CTA has left. Lane `lane` of `lanes`.
+__host__ __device__ inline void refuse_rows(uint32_t* out, int64_t pairs, uint32_t nan, float* m, int64_t parts, int lane,
+                                            int lanes) {
+  for (int64_t i = lane; i < pairs; i += lanes) out[i] = nan;
+  for (int64_t i = lane; i < parts; i += lanes) m[i] = NAN;
 }
 
 template <typename TQ, bool FP8, int D, int NG>
@@ -869,6 +877,9 @@ __global__ void __launch_bounds__(warps_of(FP8, D) * 32, AttendShape<FP8, D, NG>
     slot = slot == STAGES - 1 ? 0 : slot + 1;
   }
   cp_async_wait<0>();
+  if (!alive)
+    refuse_rows(static_cast<uint32_t*>(p.out), (int64_t)p.rows * p.H * (D / 2), Mma<TQ>::pack(NAN, NAN), ws.m,
+                ws.m ? (int64_t)p.rows * p.H * ws.parts : 0, lane, 32);
 }
 
 // Joins the parts of a row and head that has several: grid (H, rows), 256 threads; D / 4 threads a part, 1024 / D parts

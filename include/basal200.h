@@ -367,9 +367,11 @@ int basal200_constrain_logits(const void* logits, int dtype, int64_t ld, int row
 
 /* ---- Diagnostics ---- */
 
-/* Fault bits (basal200_device_faults): a bounded wait of a GEMM gave up (producer, MMA issuer, epilogue, drain), a
- * readout id or a token id was out of range, a peer barrier's wait for another rank gave up, a cache's table named a
- * page that is not there (or a row was longer than its table), or a row's state slot was out of range or taken. */
+/* Fault bits (basal200_device_faults): a bounded wait of a GEMM gave up (producer, MMA issuer, epilogue, drain; the
+ * epilogue's bit also stands for basal200_paged_attention's joins, whose warps can disagree only when the lengths are
+ * changed during the call: its rows are then NaN), a readout id or a token id was out of range, a peer barrier's wait for
+ * another rank gave up, a cache's table named a page that is not there (or a row was longer than its table), or a row's
+ * state slot was out of range or taken. */
 enum {
   BASAL200_FAULT_TIMEOUT_PRODUCER = 1,
   BASAL200_FAULT_TIMEOUT_MMA = 2,

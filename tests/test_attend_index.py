@@ -41,3 +41,21 @@ def test_every_head_that_an_item_reads_exists(tmp_path):
                        head0, head0 + heads - 1);
             }
         }""") == ""
+
+
+def test_a_wait_that_gave_up_leaves_no_row_as_it_was_allocated(tmp_path):
+    """refuse_rows, a warp's 32 lanes one after another: NaN in every value of an output and in every part's maximum, and
+    nothing past them. (A wait gives up only when a caller changes the lengths during the call.)"""
+    assert host_program(tmp_path, """
+  static uint32_t out[1000];
+  static float m[100];
+  for (int parts : {0, 1, 33, 99})
+    for (int pairs : {0, 1, 31, 64, 999}) {
+      for (auto& x : out) x = 7;
+      for (auto& x : m) x = 7.0f;
+      for (int lane = 0; lane < 32; ++lane) refuse_rows(out, pairs, 0x7FFF7FFFu, m, parts, lane, 32);
+      for (int i = 0; i < 1000; ++i)
+        if (out[i] != (i < pairs ? 0x7FFF7FFFu : 7u)) printf("pair %d of %d\\n", i, pairs);
+      for (int i = 0; i < 100; ++i)
+        if (i < parts ? m[i] == m[i] : m[i] != 7.0f) printf("part %d of %d\\n", i, parts);
+    }""") == ""
