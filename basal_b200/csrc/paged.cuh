@@ -24,15 +24,6 @@ template <>
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <>
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float widen(uint8_t v) { return e4m3_to_float(v); }
-
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 
 // x / d for 0 <= x < 2^31 by a multiplication (Granlund and Montgomery 1994): shift = ceil(log2 d), mul =
 // floor(2^32 (2^shift - d) / d) + 1, x / d = (mulhi(x, mul) + x) >> shift. Exact, and the sum stays below 2^32.
