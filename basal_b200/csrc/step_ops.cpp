@@ -193,16 +193,15 @@ void kv_copy_pages(at::TensorList pools, at::IntArrayRef src, at::IntArrayRef ds
   void* base[8];
   int layers[8];
   int64_t bytes[8];
-  bool empty = src.empty();
-  for (size_t i = 0; i < pools.size(); ++i) {
-    const Tensor& p = pools[i];
+  int held = 0;  // pools that hold anything
+  for (const Tensor& p : pools) {
     on(p, dev);
     TORCH_CHECK_VALUE(p.dim() >= 3 && p.size(1) == N && p.is_contiguous(), what,
                       ": the pools must be contiguous [layers, pages, ...] of equally many pages");
-    base[i] = ptr(p);
-    layers[i] = to_int(what, p.size(0));
-    bytes[i] = p.stride(1) * p.element_size();
-    empty |= p.numel() == 0;
+    if (p.numel() == 0) continue;
+    base[held] = ptr(p);
+    layers[held] = to_int(what, p.size(0));
+    bytes[held++] = p.stride(1) * p.element_size();
   }
   std::vector<int32_t> moves(src.size() * 2);
   for (size_t i = 0; i < src.size(); ++i) {
@@ -211,9 +210,9 @@ void kv_copy_pages(at::TensorList pools, at::IntArrayRef src, at::IntArrayRef ds
     moves[i] = (int32_t)src[i];
     moves[src.size() + i] = (int32_t)dst[i];
   }
-  if (empty) return;
+  if (!held || src.empty()) return;
   const c10::cuda::CUDAGuard guard(dev);
-  done(what, basal200_kv_copy_pages(base, layers, bytes, (int)pools.size(), N, moves.data(), moves.data() + src.size(),
+  done(what, basal200_kv_copy_pages(base, layers, bytes, held, N, moves.data(), moves.data() + src.size(),
                                     to_int(what, (int64_t)src.size()),
                                     c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
 }

@@ -564,3 +564,16 @@ def test_attention_of_values_near_the_largest(ops, fp8):
             else:
                 pool.full[i][pages, :, off] = y.to(BF)
     check(ops, pool, q, 128 ** -0.5, attend(ops, pool, q, 128 ** -0.5))
+
+
+def test_copies_beside_a_pool_that_holds_nothing(ops):
+    """A pool of no layers, or of pages of no bytes, leaves the others' copies as they are."""
+    p = torch.arange(2 * 6 * 8, dtype=torch.int32, device="cuda").view(2, 6, 8)
+    want = p.clone()
+    want[:, 4] = want[:, 1]
+    ops.kv_copy_pages([p.new_empty(0, 6, 8), p, p.new_empty(3, 6, 0)], [1], [4])
+    assert torch.equal(p, want)
+    ops.kv_copy_pages([p.new_empty(0, 6, 8)], [1], [4])
+    with pytest.raises(ValueError):
+        ops.kv_copy_pages([p.new_empty(0, 6, 8), p], [1, 1], [4, 4])
+    assert torch.equal(p, want)
