@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <vector>
@@ -347,3 +348,14 @@ TORCH_LIBRARY_FRAGMENT(basal, m) {
 
 TORCH_LIBRARY_IMPL(basal, CUDA, m) { BASAL_STEP_OPS(m); }
 TORCH_LIBRARY_IMPL(basal, CPU, m) { BASAL_STEP_OPS(m); }  // for the refusal: there is no CPU implementation
+
+// No gradients, as the package's other ops: a backward pass through an output raises (torch's default for an op from C++ is a
+// warning, and no gradient).
+#define BASAL_NO_GRADIENT(m, op) m.impl(op, torch::autograd::autogradNotImplementedFallback())
+TORCH_LIBRARY_IMPL(basal, Autograd, m) {
+  BASAL_NO_GRADIENT(m, "paged_attention");
+  BASAL_NO_GRADIENT(m, "kv_append");
+  BASAL_NO_GRADIENT(m, "kv_copy_pages");
+  BASAL_NO_GRADIENT(m, "gdn_step");
+  BASAL_NO_GRADIENT(m, "constrain_logits");
+}

@@ -544,3 +544,19 @@ def test_gdn_step_inputs_at_any_offset(ops, offset):
         assert b[name].is_contiguous()
     assert torch.equal(step(ops, b), step(ops, a))
     assert torch.equal(a["state"], b["state"]) and torch.equal(a["tail"], b["tail"])
+
+
+# --- gradients ------------------------------------------------------------------------------------------------------
+def test_a_backward_pass_is_refused(ops):
+    """With gradients on: the same outputs, and an error from a backward pass through any of them, never silence."""
+    x, y = decoder(ops), decoder(ops)
+    want = decode(ops, y)
+    for name in ("q", "new", "proj", "logits"):
+        x[name].requires_grad_()
+    outs = decode(ops, x)
+    for got, w in zip(outs, want):
+        assert torch.equal(got, w)
+        assert got.requires_grad
+        with pytest.raises(RuntimeError):
+            got.float().nan_to_num(0, 0, 0).sum().backward()
+    assert all(x[name].grad is None for name in ("q", "proj", "logits"))
