@@ -63,6 +63,14 @@ void done(const char* name, int rc) {
 }
 
 void* ptr(const Tensor& t) { return t.data_ptr(); }
+
+// A tensor that the call writes: its version counter says so, as after any torch op that writes its argument.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const OptTensor& t) {
+  if (get(t)) written(*t);
+}
 template <typename T>
 T* ptr_or_null(const OptTensor& t) {
   return get(t) ? static_cast<T*>(t->data_ptr()) : nullptr;
@@ -182,6 +190,7 @@ void kv_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, co
                                 static_cast<const int32_t*>(ptr(start)),
                                 count.defined() ? static_cast<const int32_t*>(ptr(count)) : nullptr, to_int(what, rows),
                                 to_int(what, T), c.Hk, c.D, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  written(k_pages), written(v_pages), written(ks), written(vs);
 }
 
 void kv_copy_pages(at::TensorList pools, at::IntArrayRef src, at::IntArrayRef dst) {
@@ -216,6 +225,7 @@ void kv_copy_pages(at::TensorList pools, at::IntArrayRef src, at::IntArrayRef ds
   done(what, basal200_kv_copy_pages(base, layers, bytes, held, N, moves.data(), moves.data() + src.size(),
                                     to_int(what, (int64_t)src.size()),
                                     c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  for (const Tensor& p : pools) written(p);
 }
 
 Tensor gdn_step(const Tensor& proj_in, const Tensor& tail, const Tensor& conv_in, const Tensor& A_log_in,
@@ -264,6 +274,7 @@ Tensor gdn_step(const Tensor& proj_in, const Tensor& tail, const Tensor& conv_in
                                at_slot.defined() ? static_cast<const int32_t*>(ptr(at_slot)) : nullptr, slots,
                                to_int(what, rows), (int)Hk, (int)Hv, ptr(o),
                                c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  written(tail), written(state);
   return o;
 }
 

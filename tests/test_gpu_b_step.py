@@ -560,3 +560,27 @@ def test_a_backward_pass_is_refused(ops):
         with pytest.raises(RuntimeError):
             got.float().nan_to_num(0, 0, 0).sum().backward()
     assert all(x[name].grad is None for name in ("q", "proj", "logits"))
+
+
+def test_what_the_ops_write_is_marked_as_written(ops):
+    """The version counters of the pages, their scales, the tail and the state rise, so that autograd refuses a backward pass
+    through a value it saved before; what the ops only read keeps its count. Also on tensors made under inference_mode."""
+    x = decoder(ops)
+    scales = [torch.ones(9, 2, 16, device="cuda") for _ in range(2)]
+    codes = [torch.zeros(9, 2, 16, 64, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+    wrote = [x["k"], x["v"], x["tail"], x["state"], *scales, *codes]
+    read = [x[n] for n in ("q", "new", "table", "lengths", "proj", "conv", "slots", "logits", "past")]
+    before = [t._version for t in wrote], [t._version for t in read]
+    decode(ops, x)
+    ops.kv_append(x["new"], x["new"], *codes, x["table"], x["lengths"] - 1, None, *scales)
+    assert all(t._version > n for t, n in zip(wrote, before[0]))
+    assert [t._version for t in read] == before[1]
+    w = torch.ones_like(x["state"], requires_grad=True)
+    loss = (w * x["state"]).sum()          # saves the state
+    decode(ops, x)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        y = decoder(ops)
+        decode(ops, y)
+    decode(ops, y)
