@@ -12,7 +12,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbasal200.so")
-TORCH_LIB_PATH = os.path.join(HERE, "libbasal200_torch.so")
+TORCH_LIB_PATH = os.path.join(HERE, f"libbasal200_torch-{torch.__version__}.so")  # built against this torch
 
 BF16, F16, F32, E4M3 = 0, 1, 2, 3
 DTYPE_CODE = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
@@ -92,7 +92,7 @@ def lib():
 
 
 def load_torch_ops():
-    """Loads libbasal200_torch.so, the torch ops registered in C++ (csrc/step_ops.cpp); ImportError when it was not built."""
+    """Loads the torch ops registered in C++ (csrc/step_ops.cpp); ImportError when they were not built for this torch."""
     lib()
     if not os.path.exists(TORCH_LIB_PATH):
         raise ImportError(f"{TORCH_LIB_PATH} is missing: build it with `python basal_b200/build.py`")

@@ -119,3 +119,17 @@ def test_ops_refuse_cpu_tensors():
                  (ops.constrain_logits, (z(1, 10),))):
         with pytest.raises(ValueError, match="CUDA"):
             f(*a)
+
+
+def test_the_torch_ops_are_those_of_the_installed_torch():
+    """The library that build.py writes and the one that the package loads are the same file, named after this torch: one
+    built against another torch is left alone."""
+    import importlib.util
+    import os
+
+    from basal_b200 import _lib
+    spec = importlib.util.spec_from_file_location("build_under_test", os.path.join(_lib.HERE, "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    assert build.torch_version() == torch.__version__
+    assert build.TORCH_LIB == _lib.TORCH_LIB_PATH and torch.__version__ in os.path.basename(build.TORCH_LIB)
