@@ -96,7 +96,10 @@ def load_torch_ops():
     lib()
     if not os.path.exists(TORCH_LIB_PATH):
         raise ImportError(f"{TORCH_LIB_PATH} is missing: build it with `python basal_b200/build.py`")
-    torch.ops.load_library(TORCH_LIB_PATH)
+    try:
+        torch.ops.load_library(TORCH_LIB_PATH)
+    except OSError as e:
+        raise ImportError(f"{TORCH_LIB_PATH} does not load: build it with `python basal_b200/build.py --force` ({e})") from e
 
 
 def ptr(t):

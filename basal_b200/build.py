@@ -1,7 +1,7 @@
 """Builds libbasal200.so (every CUDA kernel of the package, sm_100a only) and libbasal200_torch-<torch version>.so (the torch
 ops that are registered in C++, which call it) next to this file.
 
-    python basal_b200/build.py [--force]    (a plain script: importing basal_b200 needs the built libraries)
+    python basal_b200/build.py [--force]    (a plain script: importing basal_b200 needs libbasal200.so)
 
 nvcc cross-compiles without a GPU. libbasal200.so links the CUDA runtime statically and resolves the one driver
 function it needs (cuTensorMapEncodeTiled) at run time, so it loads wherever a CUDA 12.8+ driver is present.

@@ -630,41 +630,44 @@ def _(q, k, v, g, beta, s0, o_16bit=False):
 # ---------------------------------------------------------------------------------------------------------------
 # one new token a row: the paged key / value cache, the recurrent state, the next token's logits
 # ---------------------------------------------------------------------------------------------------------------
-# Registered in C++ (csrc/step_ops.cpp): a step's kernels run for a few microseconds, and so does a call from there.
-_lib.load_torch_ops()
-_STEP = torch.ops.basal
+# Registered in C++ (csrc/step_ops.cpp): a step's kernels run for a few microseconds, and so does a call from there. The ops
+# above need libbasal200.so alone; where the C++ ops were not built for this torch, these say so when they are called.
+try:
+    _lib.load_torch_ops()
+except ImportError as _e:
+    _why = str(_e)
 
+    def _unbuilt(*args):
+        raise ImportError(_why)
 
-@torch.library.register_fake("basal::paged_attention")
-def _(q, k_pages, v_pages, table, lengths, scale, window=0, k_scale=None, v_scale=None):
-    return q.new_empty(q.shape)
+    _paged_attention = _kv_append = _kv_copy_pages = _gdn_step = _constrain_logits = _unbuilt
+else:
+    _STEP = torch.ops.basal
+    _paged_attention = _STEP.paged_attention.default
+    _kv_append = _STEP.kv_append.default
+    _kv_copy_pages = _STEP.kv_copy_pages.default
+    _gdn_step = _STEP.gdn_step.default
+    _constrain_logits = _STEP.constrain_logits.default
 
+    @torch.library.register_fake("basal::paged_attention")
+    def _(q, k_pages, v_pages, table, lengths, scale, window=0, k_scale=None, v_scale=None):
+        return q.new_empty(q.shape)
 
-@torch.library.register_fake("basal::kv_append")
-def _(k, v, k_pages, v_pages, table, start, count=None, k_scale=None, v_scale=None):
-    return None
+    @torch.library.register_fake("basal::kv_append")
+    def _(k, v, k_pages, v_pages, table, start, count=None, k_scale=None, v_scale=None):
+        return None
 
+    @torch.library.register_fake("basal::kv_copy_pages")
+    def _(pools, src, dst):
+        return None
 
-@torch.library.register_fake("basal::kv_copy_pages")
-def _(pools, src, dst):
-    return None
+    @torch.library.register_fake("basal::gdn_step")
+    def _(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots=None):
+        return proj.new_empty((proj.shape[0], Hv, 1, 128))
 
-
-@torch.library.register_fake("basal::gdn_step")
-def _(proj, tail, conv, A_log, dt_bias, state, Hk, Hv, b_off, a_off, slots=None):
-    return proj.new_empty((proj.shape[0], Hv, 1, 128))
-
-
-@torch.library.register_fake("basal::constrain_logits")
-def _(logits, mask=None, past=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias_values=None):
-    return logits.new_empty(logits.shape, dtype=torch.float32)
-
-
-_paged_attention = _STEP.paged_attention.default
-_kv_append = _STEP.kv_append.default
-_kv_copy_pages = _STEP.kv_copy_pages.default
-_gdn_step = _STEP.gdn_step.default
-_constrain_logits = _STEP.constrain_logits.default
+    @torch.library.register_fake("basal::constrain_logits")
+    def _(logits, mask=None, past=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias_values=None):
+        return logits.new_empty(logits.shape, dtype=torch.float32)
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, scale: float,

@@ -133,3 +133,29 @@ def test_the_torch_ops_are_those_of_the_installed_torch():
     spec.loader.exec_module(build)
     assert build.torch_version() == torch.__version__
     assert build.TORCH_LIB == _lib.TORCH_LIB_PATH and torch.__version__ in os.path.basename(build.TORCH_LIB)
+
+
+@pytest.mark.parametrize("there", [False, True])
+def test_the_package_without_the_torch_ops(tmp_path, there):
+    """Without the library of the C++ ops (or with one that does not load) the package is imported and its other ops are
+    there; the five raise ImportError, with what to do, when they are called."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+
+    from basal_b200 import _lib
+    copy = tmp_path / "basal_b200"
+    shutil.copytree(_lib.HERE, copy, ignore=shutil.ignore_patterns("libbasal200_torch*", "__pycache__"))
+    if there:
+        (copy / os.path.basename(_lib.TORCH_LIB_PATH)).write_text("not a library")
+    prog = ("import torch, basal_b200\nfrom basal_b200 import ops, hybrid\nassert basal_b200.__file__.startswith(%r)\n"
+            "print(torch.ops.basal.fp8_act_quant.default)\n"
+            "for f, n in ((ops.paged_attention, 6), (ops.kv_append, 6), (ops.gdn_step, 10), (ops.constrain_logits, 1)):\n"
+            "    try:\n        f(*[None] * n)\n    except ImportError as e:\n        print('said', 'build.py' in str(e))\n"
+            "try:\n    ops.kv_copy_pages([None], [0], [1])\nexcept ImportError as e:\n    print('said', 'build.py' in str(e))\n"
+            % str(tmp_path))
+    got = subprocess.run([sys.executable, "-c", prog], cwd=tmp_path, env={**os.environ, "PYTHONPATH": str(tmp_path)},
+                         capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr
+    assert got.stdout.split("\n")[:6] == ["basal.fp8_act_quant.default"] + ["said True"] * 5
