@@ -394,17 +394,23 @@ class HybridClassifier:
         """Greedy answers of `steps` tokens after rows ids [B, S] -> int64 [B, steps]. Each step's logits (the LM head
         over the whole vocabulary) go through basal::constrain_logits with the row's answer so far as its history.
         mask: None, a bit mask [1 or B, ceil(vocab / 32)] for every step, or a function of the answer so far (int32
-        [B, t]) that returns the step's mask. repetition, presence, frequency: fp32 [B] or None."""
+        [B, t]) that returns the step's mask. repetition, presence, frequency: fp32 [B] or None. A row whose step leaves
+        no token (every logit -inf) ends there: -1 for that token and all later ones, in the answer and in what the mask
+        function sees."""
         s = self.open(ids, st, max(0, steps - 1), page_size, fp8)
         B = len(s.seqs)
         past = torch.full((B, max(1, steps)), -1, dtype=torch.int32, device=self.device)
         for t in range(steps):
             if t:
-                self.step(past[:, t - 1].long(), s)
+                self.step(past[:, t - 1].clamp(min=0).long(), s)  # a row that has ended goes on with any token
             now = mask(past[:, :t]) if callable(mask) else mask
             z = ops.constrain_logits(F.linear(s.hidden, self.head.weight), now, past, repetition, presence, frequency,
                                      bias_ids, bias_values)
-            past[:, t] = z.argmax(-1)
+            best = z.argmax(-1, keepdim=True)
+            ended = z.gather(1, best)[:, 0] == -math.inf
+            if t:
+                ended |= past[:, t - 1] < 0
+            past[:, t] = best[:, 0].masked_fill(ended, -1)
         return past[:, :steps].long()
 
     def linears(self):

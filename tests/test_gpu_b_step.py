@@ -584,3 +584,33 @@ def test_what_the_ops_write_is_marked_as_written(ops):
         y = decoder(ops)
         decode(ops, y)
     decode(ops, y)
+
+
+# --- answers and steps that the tests above leave out --------------------------------------------------------------
+def small_model(seed, vocab=777):
+    from basal_b200 import hybrid as hy
+    cfg = hy.HybridConfig(layers=4, hidden=256, heads=4, kv_heads=2, inter=256, vocab=vocab, lin_k_heads=1, lin_v_heads=2)
+    m = hy.HybridClassifier(cfg, seed=seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    st = m.prefix(torch.randint(0, vocab, (33,), device="cuda", generator=g))
+    return m, st, torch.randint(0, vocab, (2, 20), device="cuda", generator=g)
+
+
+def test_an_answer_ends_where_its_mask_leaves_nothing(ops):
+    """A row whose step allows no token gets -1 from there on; the other row's answer is the same as before."""
+    m, st, ids = small_model(5)
+    free = m.answer(ids, st, 5)
+    seen = []
+
+    def grammar(past):
+        seen.append(past.tolist())
+        mask = torch.full((2, 25), -1, dtype=torch.int32, device="cuda")
+        if past.shape[1] == 2:
+            mask[0] = 0
+        return mask
+
+    got = m.answer(ids, st, 5, mask=grammar)
+    assert got[0].tolist() == free[0, :2].tolist() + [-1] * 3 and torch.equal(got[1], free[1])
+    assert seen[4][0] == got[0, :4].tolist() and seen[4][1] == free[1, :4].tolist()
+    none = m.answer(ids, st, 3, mask=torch.zeros(1, 25, dtype=torch.int32, device="cuda"))
+    assert (none == -1).all() and none.dtype == torch.int64
