@@ -678,7 +678,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     size]; table [rows, width] int32: the page of positions j * page size ..; lengths [rows] int32, the new token's
     own position included (its key and value are appended first). Heads share key / value heads in order. A length <= 0
     gives zeros. A page that is needed and not there, or a length past the table, gives a NaN row and a fault bit. What the
-    pages hold where a row reads nothing does not matter; an infinite or NaN value that it reads makes its output NaN.
+    pages hold where a row reads nothing does not matter. An infinite or NaN value that it reads makes that dimension of the
+    heads that share it infinite or NaN; a NaN logit or one of +inf makes its head NaN; one of -inf has no weight, and
+    a row of nothing else gives zeros.
     Pages may be strided views (their last dimension contiguous, the others multiples of 16 bytes). A row's output is
     the same bits alone and among other rows."""
     return _paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)

@@ -308,8 +308,10 @@ int basal200_code_probs(const float* z, int64_t R, int64_t U, const int64_t* idx
 /* out [rows, H, D] (q_dtype bf16 or fp16, contiguous) = softmax(scale q . k_t) v over each row's positions
  * max(0, lengths[b] - window) <= t < lengths[b] (window 0: from 0). q [rows, H, D] with element strides q_row, q_head;
  * head h reads key / value head h / (H / Hk). A length <= 0 gives zeros; one above width * page_size gives NaN and
- * the fault bit. 16-bit pools have q's type. An infinite or NaN value that a row reads makes its output NaN. A row's bits do not depend on the other rows of the call. workspace
- * (16-byte aligned): basal200_paged_attention_workspace_bytes(...) bytes. */
+ * the fault bit. 16-bit pools have q's type. An infinite or NaN value that a row reads makes that dimension of the heads
+ * that share it infinite or NaN; a NaN logit or one of +inf makes its head NaN; one of -inf has no weight, and a row of
+ * nothing else gives zeros. A row's bits do not depend on the other rows of the call. workspace (16-byte aligned):
+ * basal200_paged_attention_workspace_bytes(...) bytes. */
 int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t q_head, const void* k, const void* v,
                              int kv_dtype, int64_t page_stride, int64_t head_stride, int64_t token_stride,
                              const float* ks, const float* vs, int64_t s_page, int64_t s_head, int64_t pages,

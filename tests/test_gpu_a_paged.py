@@ -577,3 +577,93 @@ def test_copies_beside_a_pool_that_holds_nothing(ops):
     with pytest.raises(ValueError):
         ops.kv_copy_pages([p.new_empty(0, 6, 8), p], [1, 1], [4, 4])
     assert torch.equal(p, want)
+
+
+# --- infinities and NaN that a row reads ---------------------------------------------------------------------------
+INF, NAN = float("inf"), float("nan")
+
+
+def without(pool, r, at):
+    """The row's keys and values in 64 bits, position `at` left out, in check()'s place of the row."""
+    class Rest(Pool):
+        def __init__(self):
+            self.scales = pool.scales
+
+        def row(self, n):
+            k, v = pool.row(r)
+            keep = torch.arange(k.shape[1], device="cuda") != at
+            return k[:, keep], v[:, keep]
+    return Rest()
+
+
+@pytest.mark.parametrize("dtype, fp8", [(BF, False), (FP16, False), (BF, True), (FP16, True)])
+@pytest.mark.parametrize("n, at", [(100, 37), (5000, 4099)])
+@pytest.mark.parametrize("what", [INF, -INF, NAN])
+def test_attention_of_keys_with_infinities(ops, dtype, fp8, n, at, what):
+    """A token of key head 1 whose key has an infinite (8-bit: a scale) or NaN part: logits of +inf and NaN make their
+    heads NaN, one of -inf leaves the token out, and neither the other key head nor the other row see any of it."""
+    pool = Pool([n, 100], 2, 128, 16, dtype, fp8, seed=41)
+    q = torch.randn(2, 4, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(42)).to(dtype)
+    q[0, 2], q[0, 3] = q[0, 2].abs() + 0.1, -q[0, 3].abs() - 0.1        # logits of both signs
+    clean = attend(ops, pool, q, 0.09)
+    page, off = pool.table[0, at // 16].long(), at % 16
+    if fp8:
+        pool.full[0].view(torch.uint8)[page, 1, off] = torch.full((128,), 0.5).to(E4M3).view(torch.uint8).cuda()
+        pool.scales[0][page, 1, off] = what
+    else:
+        pool.full[0][page, 1, off, 5] = what
+    got = attend(ops, pool, q, 0.09)
+    assert torch.equal(got[0, :2], clean[0, :2]) and torch.equal(got[1], clean[1])
+    lost = (2, 3) if what != what else (2,) if what > 0 else (3,)
+    for h in (2, 3):
+        if h in lost:
+            assert got[0, h].isnan().all()
+        else:  # check() of this head alone, over the row without the token
+            check(ops, _one_head(without(pool, 0, at), 1), q[:1, h:h + 1], 0.09, got[:1, h:h + 1])
+
+
+def _one_head(pool, head):
+    row = pool.row
+    pool.row = lambda n: tuple(x[head:head + 1] for x in row(n))
+    return pool
+
+
+@pytest.mark.parametrize("dtype, fp8", [(BF, False), (FP16, False), (BF, True), (FP16, True)])
+@pytest.mark.parametrize("n, at", [(100, 37), (5000, 4099)])
+@pytest.mark.parametrize("what", [INF, -INF, NAN])
+def test_attention_of_values_with_infinities(ops, dtype, fp8, n, at, what):
+    """A value's infinite or NaN part (8-bit: a NaN code, or the scale) reaches its dimension (the scale: every one) of the
+    heads of its key head and nothing else."""
+    pool = Pool([n, 100], 2, 128, 16, dtype, fp8, seed=43)
+    q = torch.randn(2, 4, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(44)).to(dtype)
+    clean = attend(ops, pool, q, 0.09)
+    page, off = pool.table[0, at // 16].long(), at % 16
+    dims = torch.zeros(128, dtype=torch.bool, device="cuda")
+    if not fp8:
+        pool.full[1][page, 1, off, 5] = what
+        dims[5] = True
+    elif what != what:
+        pool.full[1].view(torch.uint8)[page, 1, off, 5] = 0x7F
+        dims[5] = True
+    else:
+        pool.scales[1][page, 1, off] = what
+        dims[:] = True
+    got = attend(ops, pool, q, 0.09)
+    assert torch.equal(got[0, :2], clean[0, :2]) and torch.equal(got[1], clean[1])
+    assert not got[0, 2:][:, dims].isfinite().any()
+    assert torch.equal(got[0, 2:][:, ~dims], clean[0, 2:][:, ~dims])
+
+
+@pytest.mark.parametrize("dtype, fp8", [(BF, False), (FP16, False), (BF, True), (FP16, True)])
+def test_attention_of_nothing_but_minus_infinity(ops, dtype, fp8):
+    pool = Pool([1, 20], 1, 64, 16, dtype, fp8, seed=45)
+    q = torch.ones(2, 2, 64, dtype=dtype, device="cuda")
+    for r, size in ((0, 1), (1, 20)):
+        for t in range(size):
+            page = pool.table[r, t // 16].long()
+            if fp8:
+                pool.full[0].view(torch.uint8)[page, :, t % 16] = torch.ones(64).to(E4M3).view(torch.uint8).cuda()
+                pool.scales[0][page, :, t % 16] = -INF
+            else:
+                pool.full[0][page, :, t % 16, 3] = -INF
+    assert not attend(ops, pool, q, 0.125).any()
