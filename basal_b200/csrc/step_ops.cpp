@@ -260,7 +260,8 @@ Tensor gdn_step(const Tensor& proj_in, const Tensor& tail, const Tensor& conv_in
   }
   const c10::cuda::CUDAGuard guard(dev);
   Tensor proj = proj_in;
-  if (rows > 0 && (proj.stride(1) != 1 || proj.stride(0) % 4 || !aligned(proj, 8))) {  // rows at multiples of 16 bytes
+  const bool fits = proj.stride(1) == 1 && proj.stride(0) % 4 == 0 && (rows < 2 || proj.stride(0) >= width) && aligned(proj, 8);
+  if (rows > 0 && !fits) {  // rows at multiples of 16 bytes, one after another
     proj = at::empty({rows, (width + 7) / 8 * 8}, proj_in.options()).narrow(1, 0, width);
     proj.copy_(proj_in);
   }

@@ -648,3 +648,13 @@ def test_model_token_by_token_over_8bit_pages(ops, monkeypatch, page_size):
     for a, b, c in zip(got, want, plain):
         assert ((a - b).norm(dim=1) <= 2.0 ** -4 * b.norm(dim=1)).all()
         assert not torch.equal(b, c)
+
+
+@pytest.mark.parametrize("rows", [2, 5])
+def test_gdn_step_of_rows_that_share_memory(ops, rows):
+    """One projection expanded to every row (a row stride of 0), and rows that overlap."""
+    a, b = (inputs(rows, rows, 2, 4, BF, seed=32) for _ in range(2))
+    width = a["proj"].shape[1]
+    for view in (a["proj"][:1].expand(rows, width), torch.randn(width + 8 * rows, device="cuda").to(BF).as_strided((rows, width), (8, 1))):
+        assert torch.equal(step(ops, {**a, "proj": view}), step(ops, {**b, "proj": view.contiguous()}))
+        assert torch.equal(a["state"], b["state"]) and torch.equal(a["tail"], b["tail"])
