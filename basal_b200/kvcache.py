@@ -39,6 +39,7 @@ class Batch:
     lengths: torch.Tensor
     start: torch.Tensor
     count: torch.Tensor
+    most: int = 0  # the largest count
 
 
 class PagedKVCache:
@@ -168,12 +169,14 @@ class PagedKVCache:
             rows[i, width:] = self._length[s], self._length[s] - new, new
         t = host.to(self.device, non_blocking=True)
         lengths, start, count = t[:, width:].t().contiguous()
-        return Batch(seqs, t[:, :width], lengths, start, count)
+        return Batch(seqs, t[:, :width], lengths, start, count, max([self._new.get(s, 0) for s in seqs], default=0))
 
     def _layer(self, i):
         return (self.k[i], self.v[i]), (None, None) if self.k_scale is None else (self.k_scale[i], self.v_scale[i])
 
     def append(self, layer, batch, k, v):
+        if k.dim() > 1 and k.shape[1] < batch.most:
+            raise ValueError(f"PagedKVCache: {k.shape[1]} tokens, where grow made room for {batch.most}")
         (pk, pv), (ks, vs) = self._layer(layer)
         ops.kv_append(k, v, pk, pv, batch.table, batch.start, batch.count, ks, vs)
 

@@ -212,3 +212,19 @@ def test_no_batch_inside_a_captured_graph(moved, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="capture"):
         c.batch([a])
+
+
+def test_an_append_of_fewer_tokens_than_there_is_room_for(moved, monkeypatch):
+    """The positions behind them would be read as they were allocated; rows of uneven counts, padded, are fine."""
+    wrote = []
+    monkeypatch.setattr(kvcache.ops, "kv_append", lambda *a: wrote.append(a))
+    c = cache()
+    a, b = c.add(), c.add()
+    c.grow([a, b], [3, 2])
+    x = torch.zeros(2, 3, 1, 64)
+    with pytest.raises(ValueError, match="3"):
+        c.append(0, c.batch([a, b]), x[:, :2], x[:, :2])
+    assert not wrote
+    c.append(0, c.batch([a, b]), x, x)
+    c.append(0, c.batch([b]), x[:1, :2], x[:1, :2])
+    assert len(wrote) == 2
