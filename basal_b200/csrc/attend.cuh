@@ -1,8 +1,9 @@
 // Attention of one new token a row over a paged key / value cache (the layout is paged.cuh's):
 //   o = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t - max),  first <= t < length,
-// for the G = H / Hk query heads that share a key / value head. Every key and value is read once and used for G heads:
-// 4 G D operations on 4 D bytes (16-bit), so up to G of about 16 the bound is the cache's bytes, and the kernel is
-// built to keep enough of them in flight (96 KB an SM).
+// for the G = H / Hk query heads that share a key / value head. Every key and value is read once and used for up to 16 of
+// them (8 at D = 256); more heads are groups of that many, each an item of its own that reads them again. 4 G D
+// operations on 4 D bytes (16-bit), so up to G of about 16 the bound is the cache's bytes, and the kernel is built to keep
+// enough of them in flight (96 KB an SM).
 //
 // Work. A row's positions are cut into tiles of 16 or 32 and the tiles into items (tiles_per_item: by the row's own length,
 // so a row's sums are in the same order, and its bits the same, whatever else the call holds). A persistent CTA (of 4
@@ -11,9 +12,10 @@
 // across items: the warp that reads lengths, tables and the next item's first tiles is the one that computes the
 // current ones, and no warp waits for another but where they join an item's result. An item that is a whole row is
 // written at once; parts of longer rows go to the workspace and attend_join_kernel adds them up. Measured: 64 rows of up
-// to 8192 (16 heads over 4 of 128, 543 MB) 94 us, 89% of a copy's rate, waiting for memory; 8-bit pages, 128 rows of up to
-// 4001 (32 over 8, 541 MB) 113 us at 2 instructions a cycle an SM; one row of 200 6.5 us, of which the instructions'
-// first fetches are the larger part.
+// to 8192 (16 heads over 4 of 128, 543 MB) 94 us, 88% of a copy's rate, waiting for memory; 8-bit pages, 128 rows of up to
+// 4001 (32 over 8, 541 MB) 112 us, 74%, by the latency of the warps' own chains (11.6 warps an SM, half of the issue slots
+// and 38% of the ALU pipe in use); one row of 200 6.6 us, a warp's 1700 instructions one after another at 6.8 cycles each (of
+// them 1.9 fixed latencies, 1.6 global memory, 0.9 shared memory, 0.9 instruction fetches).
 //
 // Arithmetic, per 16 tokens: S^T [16 tokens x 8 heads] = K Q^T and O^T [D x 8 heads] += V^T P^T on mma.sync m16n8k16 with
 // fp32 accumulators (8 heads fill the n side; tcgen05 would want 64 rows or more of a tile that has G). 16-bit pages
@@ -24,11 +26,12 @@
 // fp16 while p is within 2^-16 of the largest).
 // Weights are 2^(z - ref) with z the logit times log2 e and ref a maximum that is raised only when some z passes it by
 // more than 8 (2 for fp16 pages): a tile then costs one vote instead of a maximum across lanes and a rescaling of the sums,
-// and the largest weight is 2^-8 to 1 (2^13 to 2^15), which changes no relative error (sums and outputs are fp32). An 8-bit key's scale multiplies its
-// logit, a value's scale its weight; the query and those products are brought to fp16 by powers of two of their own, the
-// head's largest query value and the largest product of a weight and a scale that it has seen (over_top), so that neither
-// the largest nor what counts beside it leaves fp16's range: a product is off by its rounding (2^-11, 2^-22 split in two) or,
-// below 2^-18 of the largest, by 2^-29 of the largest.
+// and the largest weight is 2^-8 to 1 (2^13 to 2^15), which changes no relative error (sums and outputs are fp32). An 8-bit
+// key's scale multiplies its logit, a value's scale its weight; the query and those products are brought to fp16 by powers of
+// two of their own, the head's largest query value and the largest product of a weight and a scale that it has seen
+// (over_top), so that neither the largest nor what counts beside it leaves fp16's range: a product is off by its rounding
+// (2^-11 under a bf16 output, 2^-22 split in two) or, below 2^-18 of the largest, by 2^-29 of the largest. Following the
+// products costs 5 us of the 112; splitting them under bf16 outputs too would cost 20.
 #pragma once
 #include "paged.cuh"
 

@@ -1,8 +1,8 @@
 // The torch ops for one new token a row (basal::paged_attention, kv_append, kv_copy_pages, gdn_step, constrain_logits):
 // their schemas, the checks of their tensors, and the calls of libbasal200's C ABI. Their kernels run for a few
-// microseconds at the sizes of a decoding step, where a call through torch.library and ctypes takes 25 to 30 us of host
-// time and one from here about 8, so these ops are registered in C++ (libbasal200_torch-<torch
-// version>.so, loaded by ops.py; their documentation is there).
+// microseconds at the sizes of a decoding step, where a call through torch.library and ctypes takes 25 to 32 us of host
+// time and one from here 5 to 10, so these ops are registered in C++ (libbasal200_torch-<torch version>.so, loaded by ops.py;
+// their documentation is there).
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>

@@ -682,7 +682,10 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     heads that share it infinite or NaN; a NaN logit or one of +inf makes its head NaN; one of -inf has no weight, and
     a row of nothing else gives zeros.
     Pages may be strided views (their last dimension contiguous, the others multiples of 16 bytes). A row's output is
-    the same bits alone and among other rows."""
+    the same bits alone and among other rows. Logits, weights and sums are fp32; for the products with the values a weight is
+    rounded to two 16-bit halves (off by 2^-17), or, for e4m3 pages under bf16 queries, to fp16 (2^-11: a tenth of the
+    outputs then lie on the other side of a bf16 rounding; fp16 queries get both halves). The lengths must not change
+    during the call."""
     return _paged_attention(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale)
 
 

@@ -310,8 +310,9 @@ int basal200_code_probs(const float* z, int64_t R, int64_t U, const int64_t* idx
  * head h reads key / value head h / (H / Hk). A length <= 0 gives zeros; one above width * page_size gives NaN and
  * the fault bit. 16-bit pools have q's type. An infinite or NaN value that a row reads makes that dimension of the heads
  * that share it infinite or NaN; a NaN logit or one of +inf makes its head NaN; one of -inf has no weight, and a row of
- * nothing else gives zeros. A row's bits do not depend on the other rows of the call. workspace (16-byte aligned):
- * basal200_paged_attention_workspace_bytes(...) bytes. */
+ * nothing else gives zeros. A row's bits do not depend on the other rows of the call. Logits, weights and sums are fp32; for
+ * the products with the values a weight is rounded to two 16-bit halves (off by 2^-17), or for e4m3 pools under bf16
+ * queries to fp16 (2^-11). workspace (16-byte aligned): basal200_paged_attention_workspace_bytes(...) bytes. */
 int basal200_paged_attention(const void* q, int q_dtype, int64_t q_row, int64_t q_head, const void* k, const void* v,
                              int kv_dtype, int64_t page_stride, int64_t head_stride, int64_t token_stride,
                              const float* ks, const float* vs, int64_t s_page, int64_t s_head, int64_t pages,
